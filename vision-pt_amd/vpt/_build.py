@@ -22,7 +22,10 @@ BUILD_DIAG = PKG_ROOT / "build_diag"
 LIB_DIAG = PKG_ROOT / "lib" / "libvpt_hip_diag.so"
 ARCH = "gfx950"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-CFLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Wno-unused-result"]
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 (some of their forms have given wrong results on this hardware); the host
+# pass warns that it does not know the feature, which is harmless.
+CFLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Wno-unused-result", "-Xclang", "-target-feature",
+          "-Xclang", "-packed-fp32-ops"]
 # Per-unit extra flags. gemm.hip, attention.hip: no SLP packing of f32 math into v_pk_*_f32 (packed f32 ops beside
 # MFMAs cost issue cycles: guide, 'price of one filler beside MFMAs'; attention backward -1.9 %, r05a in-process A/B).
 UNIT_FLAGS = {"gemm.hip": ["-fno-slp-vectorize"], "gemm_r2.hip": ["-fno-slp-vectorize"],
@@ -55,7 +58,7 @@ def _compile(src: Path, diag: bool = False, bdir: Path | None = None, flags: dic
     # diag/*.inc: a dependency of the units that include it (directly or through another .inc)
     incs = [f for f in sorted((CSRC / "diag").glob("*.inc")) if f.name in text] if diag else []
     incs += [f for f in sorted((CSRC / "diag").glob("*.inc")) if diag and any(f.name in i.read_text() for i in incs)]
-    deps = [src] + _headers(src) + incs
+    deps = [src, Path(__file__)] + _headers(src) + incs  # this file: the flags
     if _needs(obj, deps):
         cmd = [HIPCC, *CFLAGS, *unit_flags.get(src.name, []), *(["-DVPT_DIAG"] if diag else []), "-c", str(src), "-o",
                str(obj)]
@@ -74,14 +77,17 @@ def _gen_diag_sources() -> None:
             raise RuntimeError(f"{gen.name} failed:\n{r.stderr[-2000:]}")
 
 
-def build(verbose: bool = False, diag: bool = False) -> Path:
-    """Production library (default) or its diagnostic twin (diag=True, -DVPT_DIAG)."""
+def build(verbose: bool = False, diag: bool = False, force: bool = False) -> Path:
+    """Production library (default) or its diagnostic twin (diag=True, -DVPT_DIAG); force: every unit, also unchanged ones."""
     bdir, lib = (BUILD_DIAG, LIB_DIAG) if diag else (BUILD, LIB)
     if diag:
         _gen_diag_sources()
     bdir.mkdir(exist_ok=True)
     lib.parent.mkdir(exist_ok=True)
     srcs = sorted(CSRC.glob("*.hip"))
+    if force:
+        for src in srcs:
+            (bdir / (src.stem + ".o")).unlink(missing_ok=True)
     workers = min(len(srcs), max(1, min(8, os.cpu_count() or 1)))
     with cf.ThreadPoolExecutor(workers) as ex:
         objs = list(ex.map(lambda s: _compile(s, diag), srcs))
