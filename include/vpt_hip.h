@@ -399,6 +399,25 @@ int vpt_gemm_nf4(const void* A, long lda, const void* packed, const void* qabsma
                  const float* code2, const float* offset, long kw, int w_kmajor, const void* lora_a, long lda2,
                  const void* lora_b, long ldb2, int r, void* C, long ldc, int M, int N, int K, const void* bias,
                  const void* resid, long ldr, int out_mode, float alpha, void* stream);
+/* ---- MXFP4: microscaled 4-bit floating point ------------------------------------------------
+ * A row of K values, padded with zeros to a multiple of 128, in blocks of 32: one scale byte s per block (the values'
+ * unit is 2^(s - 127), s = max(floor(log2 max|x|) + 125, 0); 255 for a block that holds an infinity or a NaN: all its
+ * values read as NaN) and 32 codes e2m1 (sign, {0, 0.5, 1, 1.5, 2, 3, 4, 6}: nearest, ties to even, saturated at 6).
+ * codes: rows of 64 * ceil(K / 128) bytes (value 2i in the low half of byte i), row stride in bytes, a multiple of 16;
+ * scales: rows of 4 * ceil(K / 128) bytes, row stride in bytes, a multiple of 4.
+ * quantize: x [M][K], dtype 0 bf16, 1 f32, 2 f16, row stride ldx in elements. dequantize: out bf16 (exact) or f32.
+ * gemm: C[M][N] = A . B^T (+ bias[n]) (+ resid[m][n]), bf16 bias and residual, f32 accumulation and one rounding; C is
+ * bf16, or f32 with f32_out. A and B share K (the padding of both reads as zero). Any M, N, K >= 1; the fast stores need
+ * N % 8 == 0 and 16-byte rows of C and resid. M = 0 is a no-op.
+ * Stands beside the NF4 entry points above (the reference's 4-bit base: src/modules/quant/bnb.py:37-129); no interface
+ * of the reference has this format. */
+int vpt_mxfp4_quantize(const void* x, int dtype, long ldx, long M, int K, void* codes, long ldc, void* scales, long lds,
+                       void* stream);
+int vpt_mxfp4_dequantize(const void* codes, long ldc, const void* scales, long lds, long M, int K, void* out, long ldo,
+                         int f32_out, void* stream);
+int vpt_gemm_mxfp4(const void* a_codes, long lda, const void* a_scales, long ldas, const void* b_codes, long ldb,
+                   const void* b_scales, long ldbs, void* C, long ldc, int M, int N, int K, const void* bias,
+                   const void* resid, long ldr, int f32_out, void* stream);
 /* LoRA rank-16 skinny products (lora.py:92-104 lora_down / lora_up and their weight gradients):
  * lora_proj  Y[M][16] = alpha * X[M][K] . W^T, W = down [16][K] (w_kmajor = 1) or up [K][16] (0); K % 128 == 0.
  * lora_wgrad2 both adapter gradients of one LoRA Linear: g_up [N_out][16] (+)= alpha * dY^T . dS and

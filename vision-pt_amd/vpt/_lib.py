@@ -110,6 +110,9 @@ SIGNATURES: dict[str, list] = {
     "vpt_ema_update": [P, P, L, F, F, I, P],
     "vpt_gemm_nf4": [P, L, P, P, P, P, P, L, I, P, L, P, L, I, P, L, I, I, I, P, P, L, I, F, P],
     "vpt_nf4_quantize": [P, L, P, P, P, P, P, P, P],
+    "vpt_mxfp4_quantize": [P, I, L, L, I, P, L, P, L, P],
+    "vpt_mxfp4_dequantize": [P, L, P, L, L, I, P, L, I, P],
+    "vpt_gemm_mxfp4": [P, L, P, L, P, L, P, L, P, L, I, I, I, P, P, L, I, P],
     "vpt_add_bf16": [P, P, L, P, P],
     "vpt_flow_noise": [P, P, L, I, F, I, U64, P, P, P, P],
     "vpt_velocity_loss_blocks": [],

@@ -1266,3 +1266,181 @@ def cover_resize_crop(img_u8, in_h, in_w, scaled_h, scaled_w, top, left, out_h, 
     call("vpt_cover_resize_crop", img_u8.data_ptr(), in_h, in_w, scaled_h, scaled_w, top, left, out_h, out_w,
          workspace.data_ptr(), out.data_ptr(), stream())
     return out
+
+
+# ----------------------------------------------------------------------------- MXFP4 (csrc/mxfp4.hip)
+_MX_DTYPES = {BF16: 0, F32: 1, torch.float16: 2}
+
+
+def _on(dev: torch.device):
+    """The device of a call's tensors as the current one (a launch goes to the current device's stream)."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
+
+
+def _need(cond: bool, msg: str):
+    if not cond:
+        raise ValueError(msg)
+
+
+def _gpu(name: str, *ts):
+    """All of ts (None: left out) on one GPU; returns that device. Called after the checks of shapes and types."""
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        _need(t.is_cuda, f"{name}: GPU tensors expected")
+        _need(dev is None or t.device == dev, f"{name}: tensors on different devices")
+        dev = t.device
+    return dev
+
+
+def _rows2d(t, name: str, dtypes, shape=None):
+    """A [rows, cols] tensor of one of dtypes whose rows are contiguous and do not overlap."""
+    _need(t.dtype in dtypes, f"{name}: dtype {t.dtype}, expected one of {[str(d) for d in dtypes]}")
+    _need(t.dim() == 2 and (shape is None or tuple(t.shape) == tuple(shape)),
+          f"{name}: shape {tuple(t.shape)}, expected {'[rows, cols]' if shape is None else tuple(shape)}")
+    _need(t.shape[1] <= 1 or t.stride(1) == 1, f"{name}: the last dim must be contiguous")
+    _need(t.shape[0] <= 1 or t.stride(0) >= t.shape[1], f"{name}: rows must not overlap (row stride {t.stride(0)})")
+
+
+def _ld(t) -> int:
+    """The row stride of a checked [rows, cols] tensor; a single row has the stride of a dense one."""
+    return t.stride(0) if t.shape[0] > 1 else max(1, t.shape[1])
+
+
+def _vec1d(t, name: str, dtype, n: int):
+    _need(t.dtype == dtype and tuple(t.shape) == (n,) and (n <= 1 or t.stride(0) == 1),
+          f"{name}: a contiguous {dtype} [{n}] tensor expected, got {t.dtype} {tuple(t.shape)}")
+
+
+def mxfp4_shapes(rows: int, K: int) -> tuple[tuple[int, int], tuple[int, int]]:
+    """Shapes of the codes and the scales of a [rows, K] tensor: rows padded to a multiple of 128 values."""
+    steps = (K + 127) // 128
+    return (rows, 64 * steps), (rows, 4 * steps)
+
+
+def _mx_parts(codes, scales, rows, K, name: str):
+    cs, ss = mxfp4_shapes(rows, K)
+    _rows2d(codes, f"{name}: codes", (torch.uint8,), cs)
+    _rows2d(scales, f"{name}: scales", (torch.uint8,), ss)
+    _need(codes.data_ptr() % 16 == 0 and (rows <= 1 or codes.stride(0) % 16 == 0),
+          f"{name}: code rows at multiples of 16 bytes")
+    _need(scales.data_ptr() % 4 == 0 and (rows <= 1 or scales.stride(0) % 4 == 0),
+          f"{name}: scale rows at multiples of 4 bytes")
+
+
+def mxfp4_quantize(x, codes=None, scales=None):
+    """x [M, K] (bf16, f16 or f32; any K >= 1) as MXFP4: (codes u8 [M, 64 c], scales u8 [M, 4 c]), c = ceil(K / 128).
+
+    A block of 32 consecutive values of a row shares the scale 2^(s - 127), s = max(floor(log2 max|x|) + 125, 0); a code is
+    x / 2^(s - 127) rounded to the nearest of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6}, ties to the even code, saturated at 6. A block
+    with an infinity or a NaN reads back as NaN. Rows are padded with zeros to 128 values (include/vpt_hip.h)."""
+    _rows2d(x, "mxfp4_quantize: x", tuple(_MX_DTYPES))
+    M, K = x.shape
+    _need(K >= 1, "mxfp4_quantize: K >= 1")
+    cs, ss = mxfp4_shapes(M, K)
+    if codes is None:
+        codes = torch.empty(cs, dtype=torch.uint8, device=x.device)
+    if scales is None:
+        scales = torch.empty(ss, dtype=torch.uint8, device=x.device)
+    _mx_parts(codes, scales, M, K, "mxfp4_quantize")
+    dev = _gpu("mxfp4_quantize", x, codes, scales)
+    if M == 0:
+        return codes, scales
+    es = x.element_size()
+    with _on(dev):
+        _launch("mxfp4_quantize", M * K * (es + 17 / 32),
+                lambda: call("vpt_mxfp4_quantize", x.data_ptr(), _MX_DTYPES[x.dtype], _ld(x), M, K,
+                             codes.data_ptr(), _ld(codes), scales.data_ptr(), _ld(scales), stream()))
+    return codes, scales
+
+
+def mxfp4_dequantize(codes, scales, K: int, out=None, dtype=BF16):
+    """The values of an MXFP4 tensor as [M, K] bf16 (exact: a code has two significant bits) or f32."""
+    _need(K >= 1, "mxfp4_dequantize: K >= 1")
+    M = codes.shape[0]
+    _mx_parts(codes, scales, M, K, "mxfp4_dequantize")
+    if out is None:
+        _need(dtype in (BF16, F32), "mxfp4_dequantize: dtype bf16 or f32")
+        out = torch.empty(M, K, dtype=dtype, device=codes.device)
+    _rows2d(out, "mxfp4_dequantize: out", (BF16, F32), (M, K))
+    dev = _gpu("mxfp4_dequantize", codes, scales, out)
+    if M == 0:
+        return out
+    with _on(dev):
+        _launch("mxfp4_dequantize", M * K * (out.element_size() + 17 / 32),
+                lambda: call("vpt_mxfp4_dequantize", codes.data_ptr(), _ld(codes), scales.data_ptr(),
+                             _ld(scales), M, K, out.data_ptr(), _ld(out), int(out.dtype == F32), stream()))
+    return out
+
+
+def _mx_out(name, M, N, dev, bias, resid, out, out_dtype):
+    if out is None:
+        _need(out_dtype in (BF16, F32), f"{name}: out bf16 or f32")
+        out = torch.empty(M, N, dtype=out_dtype, device=dev)
+    _rows2d(out, f"{name}: out", (BF16, F32), (M, N))
+    if bias is not None:
+        _vec1d(bias, f"{name}: bias", BF16, N)
+    if resid is not None:
+        _rows2d(resid, f"{name}: resid", (BF16,), (M, N))
+    return out
+
+
+def gemm_mxfp4(a_codes, a_scales, w, out=None, *, bias=None, resid=None, out_dtype=BF16):
+    """out[M, N] = A . W^T (+ bias) (+ resid) of two MXFP4 matrices on the scaled matrix instruction: A as mxfp4_quantize
+    gives it, w a vpt.mxfp4.MXFP4Weight [N, K]. f32 accumulation, bias and residual added in f32, one rounding to out's type
+    (bf16 or f32). `out` may be `resid` itself. See csrc/mxfp4.hip."""
+    N, K = w.shape
+    M = a_codes.shape[0]
+    _mx_parts(a_codes, a_scales, M, K, "gemm_mxfp4")
+    out = _mx_out("gemm_mxfp4", M, N, a_codes.device, bias, resid, out, out_dtype)
+    dev = _gpu("gemm_mxfp4", a_codes, a_scales, w.codes, w.scales, out, bias, resid)
+    if M == 0:
+        return out
+
+    def run():
+        call("vpt_gemm_mxfp4", a_codes.data_ptr(), _ld(a_codes), a_scales.data_ptr(), _ld(a_scales),
+             w.codes.data_ptr(), _ld(w.codes), w.scales.data_ptr(), _ld(w.scales), out.data_ptr(),
+             _ld(out), M, N, K, _p(bias), _p(resid), 0 if resid is None else _ld(resid),
+             int(out.dtype == F32), stream())
+    with _on(dev):
+        _launch("gemm_mxfp4", 2.0 * M * N * K, run)
+    return out
+
+
+def linear_mxfp4(x, w, bias=None, resid=None, out=None, out_dtype=BF16):
+    """y = q(x) . W^T (+ bias) (+ resid): nn.Linear on an MXFP4 weight with its input quantised to MXFP4 on the way
+    (x [M, K] bf16, f16 or f32; w a vpt.mxfp4.MXFP4Weight [N, K]). y is bf16 or f32."""
+    _rows2d(x, "linear_mxfp4: x", tuple(_MX_DTYPES))
+    _need(x.shape[1] == w.shape[1], f"linear_mxfp4: x {tuple(x.shape)} does not match W {w.shape}")
+    out = _mx_out("linear_mxfp4", x.shape[0], w.shape[0], x.device, bias, resid, out, out_dtype)
+    dev = _gpu("linear_mxfp4", x, w.codes, w.scales, out, bias, resid)
+    if x.shape[0] == 0:
+        return out
+    with _on(dev):
+        codes, scales = mxfp4_quantize(x)
+        return gemm_mxfp4(codes, scales, w, out, bias=bias, resid=resid)
+
+
+def linear_mxfp4_dgrad(dy, w, out=None):
+    """dx = dy . W: the input gradient of linear_mxfp4, straight through the rounding of its input (dy [M, N] bf16, dx
+    [M, K] bf16). W is dequantised to bf16 (exact) and goes through the bf16 GEMM, whose rows start at multiples of 16
+    bytes: N % 8 == 0 and K % 8 == 0, and dy and out with such rows."""
+    N, K = w.shape
+    _rows2d(dy, "linear_mxfp4_dgrad: dy", (BF16,))
+    _need(dy.shape[1] == N, f"linear_mxfp4_dgrad: dy {tuple(dy.shape)} does not match W {w.shape}")
+    _need(N % 8 == 0 and K % 8 == 0, f"linear_mxfp4_dgrad: N and K multiples of 8, W {w.shape}")
+    M = dy.shape[0]
+    if out is None:
+        out = torch.empty(M, K, dtype=BF16, device=dy.device)
+    _rows2d(out, "linear_mxfp4_dgrad: out", (BF16,), (M, K))
+    for t, n in ((dy, "dy"), (out, "out")):
+        _need(t.data_ptr() % 16 == 0 and (M <= 1 or t.stride(0) % 8 == 0), f"linear_mxfp4_dgrad: {n}: 16-byte rows")
+    dev = _gpu("linear_mxfp4_dgrad", dy, w.codes, w.scales, out)
+    if M == 0:
+        return out
+    dense = lambda t: t if M > 1 else t.as_strided(t.shape, (t.shape[1], 1))  # noqa: E731 (one row: any stride)
+    with _on(dev):
+        return linear_dgrad(dense(dy), mxfp4_dequantize(w.codes, w.scales, K), out=dense(out))
