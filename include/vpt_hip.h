@@ -220,6 +220,28 @@ int vpt_qknorm_rope_bwd_rows(const void* dqk, long lddqk, const void* qkv, long 
                              int rows_per_seq, int n_valid, int D, float eps, void* stream);
 int vpt_reduce_rows(const float* in, int R, int C, float* out, int accumulate, void* stream);
 
+/* ---- the end of a gated block and the next norm, fused --------------------------------------
+ * M = groups * rows tokens of D values (D % 8 == 0, D <= 10240), group g = rows [g * rows, (g + 1) * rows):
+ *   x_out = x + resid_scale * gate * (h * rsqrt(mean h^2 + eps) * w_post)   (w_post null: h itself; gate null: 1)
+ *   y = x_out * rsqrt(mean x_out^2 + eps) * w_pre * (1 + scale) + shift      (w_pre null: no y; scale, shift null: 1, 0)
+ * y is the norm of x_out as stored. h, y bf16; x, x_out bf16, or f32 with x_f32; vectors bf16 [D] (ld 0) or one row per
+ * group (row stride ld). rstd_post / rstd_pre f32 [M] (may be null) are what the backward reads. x_out may be x.
+ * backward: dx = dx_new + the next norm's gradient, dh, and the f32 gradients of the vectors ([D], or [groups][D] dense where
+ * the vector has a row per group; each may be null), deterministic. dx_new null: zero. Without w_pre, dy, x_new, rstd_pre
+ * and dx are not used (dx is dx_new). Workspace: vpt_gated_norm_bwd_workspace bytes, 16-byte aligned, needed for the
+ * vectors' gradients. All rows at multiples of 16 bytes. The pre-norm is FP32RMSNorm (src/modules/norm.py:20-27). */
+int vpt_gated_norm_fwd(const void* h, long ldh, const void* x, int x_f32, long ldx, const void* w_post, const void* w_pre,
+                       const void* gate, long ldg, const void* scale, long lds, const void* shift, long ldsh, void* x_out,
+                       long ldxo, void* y, long ldy, float* rstd_post, float* rstd_pre, int groups, int rows, int D,
+                       float resid_scale, float eps, void* stream);
+long vpt_gated_norm_bwd_workspace(int groups, int rows, int D);
+int vpt_gated_norm_bwd(const void* dy, long lddy, const void* dx_new, long lddxn, const void* h, long ldh,
+                       const void* x_new, int x_f32, long ldxn, const float* rstd_post, const float* rstd_pre,
+                       const void* w_post, const void* w_pre, const void* gate, long ldg, const void* scale, long lds,
+                       const void* shift, long ldsh, void* dh, long lddh, void* dx, long lddx, float* dw_post,
+                       float* dw_pre, float* dgate, float* dscale, float* dshift, void* workspace, int groups, int rows,
+                       int D, float resid_scale, void* stream);
+
 /* ---- flow matching input / loss ----------------------------------------------------------------
  * patchify: z = t*x + (1-t)*eps (eps from `noise` fp16 or the counter RNG `seed`), written in the
  * Conv2d(k=16,s=16) im2col order; in_kind 1 copies a bf16 image. Replaces
@@ -320,6 +342,21 @@ int vpt_radam_sf_step(void* y, const void* grad, int grad_bf16, float* z, float*
 int vpt_grad_norm_blocks(void);
 int vpt_grad_sumsq(const void* g, int g_bf16, long n, float scale, float* part, void* stream);
 int vpt_clip_coef(const float* part, int n, float max_norm, float* coef, float* norm_out, void* stream);
+/* The global norm of many gradient tensors and their clipping (after_backward, src/models/for_training.py:98-109), for
+ * gradients in tensors of their own: the caller cuts them into pieces of at most vpt_grad_list_piece() values and keeps the
+ * table in device memory. norm: part[vpt_grad_list_parts(count)] = sums of squares (f64, fixed order). clip: norm_out (may be
+ * null) = sqrt(sum of part's `parts` sums, of this table or of another); out = clamp(min(1, max_norm / (norm + 1e-6)) * g, +-clip_value), max_norm / clip_value 0: off;
+ * out may be g. g and out of a piece have its dtype (0 bf16, 1 f32, 2 f16) and alignment. */
+typedef struct {
+  const void* g;
+  void* out;
+  int n, dtype;
+} VptGradPiece;
+int vpt_grad_list_piece(void);
+int vpt_grad_list_parts(int count);
+int vpt_grad_list_norm(const void* pieces, int count, double* part, void* stream);
+int vpt_grad_list_clip(const void* pieces, int count, const double* part, int parts, float max_norm, float clip_value,
+                       float* norm_out, void* stream);
 int vpt_sf_lerp(void* y, const float* z, long n, float w, void* stream);
 /* EMA copy of the flat bf16 parameters (swa_utils.AveragedModel(get_ema_avg_fn(decay)), use_buffers=False;
  * src/trainer/common.py:211-216, 385-386): first = 1 copies, else ema = bf16(bf16(d*ema) + bf16(omd*p)); omd = the caller's

@@ -1,0 +1,536 @@
+// The end of a gated transformer block and the norm of the next one, fused, forward and backward, for gfx950.
+//
+//   u  = h r_h w_post,  r_h = rsqrt(mean h^2 + eps)      (the norm behind the block; u = h without w_post)
+//   x' = x + s gate u                                    (gate: one vector, one per group of rows, or none)
+//   n  = x' r_x,        r_x = rsqrt(mean x'^2 + eps)     (the next block's norm, of x' as it is stored)
+//   y  = n w_pre (1 + scale) + shift                     (modulation: one vector, one per group of rows, or none)
+// Backward, from dy and the gradient dx' that the stream brings from later blocks:
+//   dn = dy (1 + scale) w_pre,  dX = dx' + r_x (dn - n mean(dn n)),  dx = dX
+//   v  = h r_h,  du = s gate dX,  dv = du w_post,  dh = r_h (dv - v mean(dv v))
+// and, per group, the column sums S = sum dy, P = sum dy n, Q = sum dX v, from which
+//   dshift = S, dscale = w_pre P, dw_pre = sum over groups (1 + scale) P,
+//   dgate = s w_post Q, dw_post = s sum over groups gate Q.
+// Beside RMSNorm (norm.hip; FP32RMSNorm, reference src/modules/norm.py:20-27), which has neither gate nor modulation.
+//
+// Both directions are bound by HBM: h, x, x', y once each forward; dy, dx', h, x', dx, dh once each backward. A row is held
+// in registers by TPR lanes, NC chunks of 8 columns per lane, so nothing is read twice; the means are sums of f32 squares
+// over at most 8 NC values per lane and then a tree over the lanes.
+#include "common.h"
+
+namespace {
+
+struct GnArgs {
+  const bf16_t* h; long ldh;
+  const void* x; long ldx;        // forward: x; backward: x'
+  void* xo; long ldxo;            // forward: x'; backward: dx
+  bf16_t* y; long ldy;            // forward: y; backward: dh
+  const bf16_t* dy; long lddy;    // backward
+  const void* dxn; long lddxn;    // backward: dx' (may be null: zero)
+  const bf16_t* w_post; const bf16_t* w_pre;
+  const bf16_t* gate; long ldg;   // row stride per group; 0: one vector for all
+  const bf16_t* scale; long lds;
+  const bf16_t* shift; long ldsh;
+  float* rstd_post; float* rstd_pre;
+  float* part;                    // backward: [groups * bpg][3][D]
+  int rows, D;                    // rows per group
+  int bpg, rpb;                   // blocks per group, rows per block
+  float s, eps;
+};
+
+template <bool F32>
+__device__ __forceinline__ void gn_load8(const void* p, long at, float (&f)[8]) {
+  if (F32) {
+    const floatx4 a = *reinterpret_cast<const floatx4*>(reinterpret_cast<const float*>(p) + at);
+    const floatx4 b = *reinterpret_cast<const floatx4*>(reinterpret_cast<const float*>(p) + at + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = a[e], f[4 + e] = b[e];
+  } else {
+    unpack8(*reinterpret_cast<const uint4*>(reinterpret_cast<const bf16_t*>(p) + at), f);
+  }
+}
+// Stores f and leaves in f the stored values.
+template <bool F32>
+__device__ __forceinline__ void gn_store8(void* p, long at, float (&f)[8]) {
+  if (F32) {
+    *reinterpret_cast<floatx4*>(reinterpret_cast<float*>(p) + at) = floatx4{f[0], f[1], f[2], f[3]};
+    *reinterpret_cast<floatx4*>(reinterpret_cast<float*>(p) + at + 4) = floatx4{f[4], f[5], f[6], f[7]};
+  } else {
+    const uint4 v = pack8(f);
+    *reinterpret_cast<uint4*>(reinterpret_cast<bf16_t*>(p) + at) = v;
+    unpack8(v, f);
+  }
+}
+
+// Sum over the TPR lanes (a power of two, at most 64) of a row, or over the whole block (TPR = 256) through `red`.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+#pragma unroll
+  for (int o = 1; o < (TPR < 64 ? TPR : 64); o <<= 1) v += __shfl_xor(v, o, 64);
+  if (TPR > 64) {
+    __syncthreads();  // the previous sum's readers are done with red
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = (red[0] + red[1]) + (red[2] + red[3]);
+  }
+  return v;
+}
+
+template <int TPR, int NC, bool XF32>
+__global__ __launch_bounds__(256) void gated_norm_fwd_kernel(GnArgs g) {
+  __shared__ float red[4];
+  constexpr int RPB = 256 / TPR;  // rows a block works on at once
+  const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  const int group = blockIdx.x / g.bpg, r0 = (blockIdx.x % g.bpg) * g.rpb;
+  const int nch = g.D >> 3;
+  const float inv = 1.f / (float)g.D;
+  const int r1 = min(g.rows, r0 + g.rpb);
+  for (int rb = r0; rb < r1; rb += RPB) {  // the same trip count for the whole block (row_sum's barriers)
+    const bool ok = rb + sub < r1;
+    const long row = (long)group * g.rows + rb + sub;
+    float u[NC][8], f[NC][8];
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = lane + TPR * i;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) u[i][e] = f[i][e] = 0.f;
+      if (ok && c < nch) {
+        gn_load8<false>(g.h, row * g.ldh + c * 8, u[i]);
+        gn_load8<XF32>(g.x, row * g.ldx + c * 8, f[i]);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss += u[i][e] * u[i][e];
+    }
+    float r = g.s;
+    if (g.w_post) {
+      const float rh = rsqrtf(row_sum<TPR>(ss, red) * inv + g.eps);
+      if (lane == 0 && ok && g.rstd_post) g.rstd_post[row] = rh;
+      r *= rh;
+    }
+    ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = lane + TPR * i;
+      if (c < nch) {
+        float t[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[i][e] *= r;
+        if (g.w_post) {
+          gn_load8<false>(g.w_post, c * 8, t);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) u[i][e] *= t[e];
+        }
+        if (g.gate) {
+          gn_load8<false>(g.gate, group * g.ldg + c * 8, t);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) u[i][e] *= t[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[i][e] += u[i][e];
+        if (ok) gn_store8<XF32>(g.xo, row * g.ldxo + c * 8, f[i]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss += f[i][e] * f[i][e];
+      }
+    }
+    if (!g.w_pre) continue;
+    const float rx = rsqrtf(row_sum<TPR>(ss, red) * inv + g.eps);
+    if (lane == 0 && ok && g.rstd_pre) g.rstd_pre[row] = rx;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = lane + TPR * i;
+      if (c < nch) {
+        float t[8];
+        gn_load8<false>(g.w_pre, c * 8, t);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[i][e] = f[i][e] * rx * t[e];
+        if (g.scale) {
+          float b[8];
+          gn_load8<false>(g.scale, group * g.lds + c * 8, t);
+          gn_load8<false>(g.shift, group * g.ldsh + c * 8, b);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[i][e] = f[i][e] * (1.f + t[e]) + b[e];
+        }
+        if (ok) gn_store8<false>(g.y, row * g.ldy + c * 8, f[i]);
+      }
+    }
+  }
+}
+
+// The rows of a block belong to one group; each lane keeps the sums S, P, Q of its columns and the block leaves one partial
+// row of each in g.part (no atomics: the same bits every time).
+template <int TPR, int NC, bool XF32>
+__global__ __launch_bounds__(256) void gated_norm_bwd_kernel(GnArgs g) {
+  extern __shared__ __attribute__((aligned(16))) float cols[];  // [D], for the block's column sums
+  __shared__ float red[4];
+  constexpr int RPB = 256 / TPR;
+  const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  const int group = blockIdx.x / g.bpg, r0 = (blockIdx.x % g.bpg) * g.rpb;
+  const int nch = g.D >> 3;
+  const float inv = 1.f / (float)g.D;
+  const int r1 = min(g.rows, r0 + g.rpb);
+  float S[NC][8], P[NC][8], Q[NC][8];
+#pragma unroll
+  for (int i = 0; i < NC; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) S[i][e] = P[i][e] = Q[i][e] = 0.f;
+  for (int rb = r0; rb < r1; rb += RPB) {
+    const bool ok = rb + sub < r1;
+    const long row = (long)group * g.rows + rb + sub;
+    float dX[NC][8], n[NC][8], dn[NC][8];
+    const float rx = ok && g.w_pre ? g.rstd_pre[row] : 0.f, rh = g.w_post ? (ok ? g.rstd_post[row] : 0.f) : 1.f;
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = lane + TPR * i;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dX[i][e] = n[i][e] = dn[i][e] = 0.f;
+      if (ok && c < nch) {
+        if (g.dxn) gn_load8<XF32>(g.dxn, row * g.lddxn + c * 8, dX[i]);
+        if (g.w_pre) {
+          float t[8];
+          gn_load8<XF32>(g.x, row * g.ldx + c * 8, n[i]);
+          gn_load8<false>(g.dy, row * g.lddy + c * 8, dn[i]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            n[i][e] *= rx;
+            S[i][e] += dn[i][e];
+            P[i][e] += dn[i][e] * n[i][e];
+          }
+          if (g.scale) {
+            gn_load8<false>(g.scale, group * g.lds + c * 8, t);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dn[i][e] *= 1.f + t[e];
+          }
+          gn_load8<false>(g.w_pre, c * 8, t);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            dn[i][e] *= t[e];
+            dot += dn[i][e] * n[i][e];
+          }
+        }
+      }
+    }
+    if (g.w_pre) {
+      const float mean = row_sum<TPR>(dot, red) * inv;
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dX[i][e] += rx * (dn[i][e] - n[i][e] * mean);
+    }
+    // n, dn are free: n = v, dn = dv
+    dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = lane + TPR * i;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) n[i][e] = dn[i][e] = 0.f;
+      if (ok && c < nch) {
+        float t[8];
+        gn_load8<false>(g.h, row * g.ldh + c * 8, n[i]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          n[i][e] *= rh;
+          Q[i][e] += dX[i][e] * n[i][e];
+          dn[i][e] = dX[i][e] * g.s;
+        }
+        if (g.gate) {
+          gn_load8<false>(g.gate, group * g.ldg + c * 8, t);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) dn[i][e] *= t[e];
+        }
+        if (g.w_post) {
+          gn_load8<false>(g.w_post, c * 8, t);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            dn[i][e] *= t[e];
+            dot += dn[i][e] * n[i][e];
+          }
+        }
+        if (g.xo) gn_store8<XF32>(g.xo, row * g.ldxo + c * 8, dX[i]);
+      }
+    }
+    const float mean = g.w_post ? row_sum<TPR>(dot, red) * inv : 0.f;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = lane + TPR * i;
+      if (ok && c < nch) {
+        if (g.w_post) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) dn[i][e] = rh * (dn[i][e] - n[i][e] * mean);
+        }
+        gn_store8<false>(g.y, row * g.ldy + c * 8, dn[i]);
+      }
+    }
+  }
+  if (!g.part) return;
+  // column sums: the lanes of a wave that hold the same columns, then the waves in order through LDS
+  float* out = g.part + (long)blockIdx.x * 3 * g.D;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    float(&A)[NC][8] = k == 0 ? S : k == 1 ? P : Q;
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int o = TPR; o < 64; o <<= 1) A[i][e] += __shfl_xor(A[i][e], o, 64);
+    if (TPR == 256) {  // every column has one lane
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const int c = lane + TPR * i;
+        if (c < nch)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) out[k * g.D + c * 8 + e] = A[i][e];
+      }
+      continue;
+    }
+    for (int w = 0; w < 4; ++w) {
+      __syncthreads();
+      if ((int)threadIdx.x >> 6 == w && (threadIdx.x & 63) < TPR) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          const int c = lane + TPR * i;
+          if (c < nch)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              if (w == 0) cols[c * 8 + e] = A[i][e];
+              else if (w < 3) cols[c * 8 + e] += A[i][e];
+              else out[k * g.D + c * 8 + e] = cols[c * 8 + e] + A[i][e];
+            }
+        }
+      }
+    }
+  }
+}
+
+struct GnSum {
+  const float* part;  // [groups * bpg][3][D]
+  float* tot;         // [groups][3][D]
+  const bf16_t* w_post; const bf16_t* w_pre;
+  const bf16_t* gate; long ldg;
+  const bf16_t* scale; long lds;
+  float* dw_post; float* dw_pre;
+  float* dgate; float* dscale; float* dshift;
+  int groups, bpg, D, gate_each, scale_each, shift_each;  // *_each: a gradient row per group
+  float s;
+};
+
+// tot[group][k][c] = sum over the group's blocks: 16 columns x 16 row slots per block, then a tree.
+__global__ __launch_bounds__(256) void gated_norm_sum_kernel(GnSum g) {
+  __shared__ float red[16][17];
+  const int cl = threadIdx.x & 15, rg = threadIdx.x >> 4;
+  const int c = blockIdx.x * 16 + cl, k = blockIdx.y, group = blockIdx.z;
+  float s = 0.f;
+  if (c < g.D)
+    for (int b = rg; b < g.bpg; b += 16) s += g.part[(((long)group * g.bpg + b) * 3 + k) * g.D + c];
+  red[rg][cl] = s;
+  __syncthreads();
+#pragma unroll
+  for (int st = 8; st >= 1; st >>= 1) {
+    if (rg < st) red[rg][cl] += red[rg + st][cl];
+    __syncthreads();
+  }
+  if (rg == 0 && c < g.D) g.tot[((long)group * 3 + k) * g.D + c] = red[0][cl];
+}
+
+// The gradients of the vectors from the groups' sums: 16 columns x 16 group slots per block, then a tree over the slots for
+// what all groups share.
+__global__ __launch_bounds__(256) void gated_norm_vec_kernel(GnSum g) {
+  __shared__ float red[5][16][17];
+  const int cl = threadIdx.x & 15, rg = threadIdx.x >> 4;
+  const int c = blockIdx.x * 16 + cl;
+  float a[5] = {0.f, 0.f, 0.f, 0.f, 0.f};  // dw_post, dw_pre, dgate, dscale, dshift
+  if (c < g.D) {
+    const float wp = g.w_post ? bf2f(g.w_post[c]) : 1.f, wn = g.w_pre ? bf2f(g.w_pre[c]) : 1.f;
+    for (int i = rg; i < g.groups; i += 16) {
+      const float* t = g.tot + (long)i * 3 * g.D + c;
+      const float S = t[0], P = t[g.D], Q = t[2 * g.D];
+      const float sc = g.scale ? bf2f(g.scale[i * g.lds + c]) : 0.f, gt = g.gate ? bf2f(g.gate[i * g.ldg + c]) : 1.f;
+      const float dg = g.s * wp * Q, ds = wn * P;
+      if (g.dgate && g.gate_each) g.dgate[(long)i * g.D + c] = dg;
+      if (g.dscale && g.scale_each) g.dscale[(long)i * g.D + c] = ds;
+      if (g.dshift && g.shift_each) g.dshift[(long)i * g.D + c] = S;
+      a[0] += g.s * gt * Q;
+      a[1] += (1.f + sc) * P;
+      a[2] += dg;
+      a[3] += ds;
+      a[4] += S;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 5; ++k) red[k][rg][cl] = a[k];
+  __syncthreads();
+#pragma unroll
+  for (int st = 8; st >= 1; st >>= 1) {
+    if (rg < st)
+#pragma unroll
+      for (int k = 0; k < 5; ++k) red[k][rg][cl] += red[k][rg + st][cl];
+    __syncthreads();
+  }
+  if (rg != 0 || c >= g.D) return;
+  if (g.dw_post) g.dw_post[c] = red[0][0][cl];
+  if (g.dw_pre) g.dw_pre[c] = red[1][0][cl];
+  if (g.dgate && !g.gate_each) g.dgate[c] = red[2][0][cl];
+  if (g.dscale && !g.scale_each) g.dscale[c] = red[3][0][cl];
+  if (g.dshift && !g.shift_each) g.dshift[c] = red[4][0][cl];
+}
+
+constexpr int kGnMaxD = 10240;
+
+// Lanes per row: the fewest of 16, 32, 64, 256 that hold the row in at most 5 chunks each.
+int gn_tpr(int D) {
+  const int nch = D / 8;
+  return nch <= 80 ? 16 : nch <= 160 ? 32 : nch <= 320 ? 64 : 256;
+}
+
+int gn_blocks_per_group(int groups, int rows, int D) {
+  const int rpb = 256 / gn_tpr(D);
+  const long want = ((long)rows + 4 * rpb - 1) / (4 * rpb), most = groups >= 1024 ? 1 : 1024 / groups;
+  return (int)(want < most ? (want < 1 ? 1 : want) : most);
+}
+
+template <int TPR, int NC>
+void gn_launch(const GnArgs& g, int blocks, bool bwd, bool xf32, hipStream_t s) {
+  const size_t lds = TPR == 256 ? 0 : (size_t)g.D * sizeof(float);
+  if (bwd && xf32) hipLaunchKernelGGL((gated_norm_bwd_kernel<TPR, NC, true>), dim3(blocks), dim3(256), lds, s, g);
+  else if (bwd) hipLaunchKernelGGL((gated_norm_bwd_kernel<TPR, NC, false>), dim3(blocks), dim3(256), lds, s, g);
+  else if (xf32) hipLaunchKernelGGL((gated_norm_fwd_kernel<TPR, NC, true>), dim3(blocks), dim3(256), 0, s, g);
+  else hipLaunchKernelGGL((gated_norm_fwd_kernel<TPR, NC, false>), dim3(blocks), dim3(256), 0, s, g);
+}
+
+template <int TPR>
+void gn_chunks(const GnArgs& g, int blocks, bool bwd, bool xf32, hipStream_t s) {
+  const int nc = (g.D / 8 + TPR - 1) / TPR;
+  if (nc <= 1) gn_launch<TPR, 1>(g, blocks, bwd, xf32, s);
+  else if (nc == 2) gn_launch<TPR, 2>(g, blocks, bwd, xf32, s);
+  else if (nc == 3) gn_launch<TPR, 3>(g, blocks, bwd, xf32, s);
+  else if (nc == 4) gn_launch<TPR, 4>(g, blocks, bwd, xf32, s);
+  else gn_launch<TPR, 5>(g, blocks, bwd, xf32, s);
+}
+
+void gn_dispatch(const GnArgs& g, int blocks, bool bwd, bool xf32, hipStream_t s) {
+  switch (gn_tpr(g.D)) {
+    case 16: gn_chunks<16>(g, blocks, bwd, xf32, s); break;
+    case 32: gn_chunks<32>(g, blocks, bwd, xf32, s); break;
+    case 64: gn_chunks<64>(g, blocks, bwd, xf32, s); break;
+    default: gn_chunks<256>(g, blocks, bwd, xf32, s);
+  }
+}
+
+bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+// Rows of D elements of es bytes at multiples of 16 bytes; a null p is no tensor.
+bool rows_ok(const void* p, long ld, int D, int es, long rows) {
+  return !p || (al16(p) && (rows <= 1 || (ld >= D && ld * es % 16 == 0)));
+}
+bool vec_ok(const void* p, long ld, int D) { return !p || (al16(p) && (ld == 0 || (ld >= D && ld % 8 == 0))); }
+
+}  // namespace
+
+extern "C" long vpt_gated_norm_bwd_workspace(int groups, int rows, int D) {
+  if (groups <= 0 || rows <= 0 || D <= 0 || D % 8 || D > kGnMaxD) return 0;
+  return ((long)groups * gn_blocks_per_group(groups, rows, D) + groups) * 3 * D * (long)sizeof(float);
+}
+
+#define VPT_GN_SHAPE(name)                                                                                             \
+  VPT_CHECK_ARG(groups >= 0 && rows >= 0 && (long)groups * rows < (1L << 31), name ": groups, rows >= 0, groups * rows < 2^31"); \
+  VPT_CHECK_ARG(D > 0 && D % 8 == 0 && D <= kGnMaxD, name ": D a multiple of 8, at most 10240");                       \
+  VPT_CHECK_ARG(!scale == !shift, name ": scale and shift go together");                                               \
+  VPT_CHECK_ARG(w_pre || !scale, name ": a modulation needs w_pre")
+
+extern "C" int vpt_gated_norm_fwd(const void* h, long ldh, const void* x, int x_f32, long ldx, const void* w_post,
+                                  const void* w_pre, const void* gate, long ldg, const void* scale, long lds,
+                                  const void* shift, long ldsh, void* x_out, long ldxo, void* y, long ldy,
+                                  float* rstd_post, float* rstd_pre, int groups, int rows, int D, float resid_scale,
+                                  float eps, void* stream) {
+  VPT_GN_SHAPE("vpt_gated_norm_fwd");
+  const long M = (long)groups * rows;
+  if (M == 0) return VPT_OK;
+  const int es = x_f32 ? 4 : 2;
+  VPT_CHECK_ARG(h && x && x_out && (!w_pre == !y), "vpt_gated_norm_fwd: h, x, x_out, and y with w_pre");
+  VPT_CHECK_ARG(rows_ok(h, ldh, D, 2, M) && rows_ok(x, ldx, D, es, M) && rows_ok(x_out, ldxo, D, es, M) &&
+                    rows_ok(y, ldy, D, 2, M),
+                "vpt_gated_norm_fwd: rows of D elements at multiples of 16 bytes");
+  VPT_CHECK_ARG(vec_ok(w_post, 0, D) && vec_ok(w_pre, 0, D) && vec_ok(gate, ldg, D) && vec_ok(scale, lds, D) &&
+                    vec_ok(shift, ldsh, D),
+                "vpt_gated_norm_fwd: vectors at multiples of 16 bytes");
+  GnArgs g{};
+  g.h = (const bf16_t*)h; g.ldh = ldh;
+  g.x = x; g.ldx = ldx;
+  g.xo = x_out; g.ldxo = ldxo;
+  g.y = (bf16_t*)y; g.ldy = ldy;
+  g.w_post = (const bf16_t*)w_post; g.w_pre = (const bf16_t*)w_pre;
+  g.gate = (const bf16_t*)gate; g.ldg = ldg;
+  g.scale = (const bf16_t*)scale; g.lds = lds;
+  g.shift = (const bf16_t*)shift; g.ldsh = ldsh;
+  g.rstd_post = rstd_post; g.rstd_pre = rstd_pre;
+  g.rows = rows; g.D = D;
+  g.rpb = 256 / gn_tpr(D);
+  g.bpg = (rows + g.rpb - 1) / g.rpb;
+  g.s = resid_scale; g.eps = eps;
+  gn_dispatch(g, groups * g.bpg, false, x_f32 != 0, (hipStream_t)stream);
+  VPT_LAUNCH_CHECK();
+  return VPT_OK;
+}
+
+extern "C" int vpt_gated_norm_bwd(const void* dy, long lddy, const void* dx_new, long lddxn, const void* h, long ldh,
+                                  const void* x_new, int x_f32, long ldxn, const float* rstd_post, const float* rstd_pre,
+                                  const void* w_post, const void* w_pre, const void* gate, long ldg, const void* scale,
+                                  long lds, const void* shift, long ldsh, void* dh, long lddh, void* dx, long lddx,
+                                  float* dw_post, float* dw_pre, float* dgate, float* dscale, float* dshift, void* workspace,
+                                  int groups, int rows, int D, float resid_scale, void* stream) {
+  VPT_GN_SHAPE("vpt_gated_norm_bwd");
+  const long M = (long)groups * rows;
+  const int es = x_f32 ? 4 : 2;
+  VPT_CHECK_ARG((w_post || !dw_post) && (w_pre || !dw_pre) && (gate || !dgate) && (scale || (!dscale && !dshift)),
+                "vpt_gated_norm_bwd: a gradient of a vector that is not there");
+  VPT_CHECK_ARG(vec_ok(w_post, 0, D) && vec_ok(w_pre, 0, D) && vec_ok(gate, ldg, D) && vec_ok(scale, lds, D) &&
+                    vec_ok(shift, ldsh, D),
+                "vpt_gated_norm_bwd: vectors at multiples of 16 bytes");
+  const bool sums = dw_post || dw_pre || dgate || dscale || dshift;
+  hipStream_t st = (hipStream_t)stream;
+  GnSum z{};
+  z.w_post = (const bf16_t*)w_post; z.w_pre = (const bf16_t*)w_pre;
+  z.gate = (const bf16_t*)gate; z.ldg = ldg;
+  z.scale = (const bf16_t*)scale; z.lds = lds;
+  z.dw_post = dw_post; z.dw_pre = dw_pre;
+  z.dgate = dgate; z.dscale = dscale; z.dshift = dshift;
+  z.groups = groups; z.D = D;
+  z.gate_each = ldg != 0; z.scale_each = lds != 0; z.shift_each = ldsh != 0;
+  z.s = resid_scale;
+  VPT_CHECK_ARG(groups <= 65535, "vpt_gated_norm_bwd: at most 65535 groups");
+  VPT_CHECK_ARG(M > 0 || !sums, "vpt_gated_norm_bwd: no rows to sum over");
+  if (M == 0) return VPT_OK;
+  VPT_CHECK_ARG(h && dh && (!w_post || rstd_post) && (!w_pre || (dy && x_new && rstd_pre && dx)) && (w_pre || dx_new),
+                "vpt_gated_norm_bwd: h, dh; rstd_post with w_post; dy, x_new, rstd_pre and dx with w_pre, dx_new without");
+  VPT_CHECK_ARG(rows_ok(dy, lddy, D, 2, M) && rows_ok(dx_new, lddxn, D, es, M) && rows_ok(h, ldh, D, 2, M) &&
+                    rows_ok(x_new, ldxn, D, es, M) && rows_ok(dh, lddh, D, 2, M) && rows_ok(dx, lddx, D, es, M),
+                "vpt_gated_norm_bwd: rows of D elements at multiples of 16 bytes");
+  VPT_CHECK_ARG(!sums || (workspace && al16(workspace)), "vpt_gated_norm_bwd: the vectors' gradients need the workspace");
+  GnArgs g{};
+  g.h = (const bf16_t*)h; g.ldh = ldh;
+  g.x = x_new; g.ldx = ldxn;
+  g.xo = w_pre ? dx : nullptr; g.ldxo = lddx;  // without a next norm dx is dx_new itself
+  g.y = (bf16_t*)dh; g.ldy = lddh;
+  g.dy = (const bf16_t*)dy; g.lddy = lddy;
+  g.dxn = dx_new; g.lddxn = lddxn;
+  g.w_post = z.w_post; g.w_pre = z.w_pre;
+  g.gate = z.gate; g.ldg = ldg;
+  g.scale = z.scale; g.lds = lds;
+  g.rstd_post = const_cast<float*>(rstd_post); g.rstd_pre = const_cast<float*>(rstd_pre);
+  g.rows = rows; g.D = D; g.s = resid_scale;
+  g.bpg = gn_blocks_per_group(groups, rows, D);
+  g.rpb = (rows + g.bpg - 1) / g.bpg;
+  g.part = sums ? (float*)workspace : nullptr;
+  const int blocks = groups * g.bpg;
+  gn_dispatch(g, blocks, true, x_f32 != 0, st);
+  VPT_LAUNCH_CHECK();
+  if (!sums) return VPT_OK;
+  z.bpg = g.bpg;
+  z.part = g.part;
+  z.tot = g.part + (long)blocks * 3 * D;
+  hipLaunchKernelGGL(gated_norm_sum_kernel, dim3((D + 15) / 16, 3, groups), dim3(256), 0, st, z);
+  VPT_LAUNCH_CHECK();
+  hipLaunchKernelGGL(gated_norm_vec_kernel, dim3((D + 15) / 16), dim3(256), 0, st, z);
+  VPT_LAUNCH_CHECK();
+  return VPT_OK;
+}

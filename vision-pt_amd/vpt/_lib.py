@@ -110,6 +110,14 @@ SIGNATURES: dict[str, list] = {
     "vpt_ema_update": [P, P, L, F, F, I, P],
     "vpt_gemm_nf4": [P, L, P, P, P, P, P, L, I, P, L, P, L, I, P, L, I, I, I, P, P, L, I, F, P],
     "vpt_nf4_quantize": [P, L, P, P, P, P, P, P, P],
+    "vpt_gated_norm_fwd": [P, L, P, I, L, P, P, P, L, P, L, P, L, P, L, P, L, P, P, I, I, I, F, F, P],
+    "vpt_gated_norm_bwd_workspace": [I, I, I],
+    "vpt_gated_norm_bwd": [P, L, P, L, P, L, P, I, L, P, P, P, P, P, L, P, L, P, L, P, L, P, L, P, P, P, P, P, P, I, I, I,
+                           F, P],
+    "vpt_grad_list_piece": [],
+    "vpt_grad_list_parts": [I],
+    "vpt_grad_list_norm": [P, I, P, P],
+    "vpt_grad_list_clip": [P, I, P, I, F, F, P, P],
     "vpt_mxfp4_quantize": [P, I, L, L, I, P, L, P, L, P],
     "vpt_mxfp4_dequantize": [P, L, P, L, L, I, P, L, I, P],
     "vpt_gemm_mxfp4": [P, L, P, L, P, L, P, L, P, L, I, I, I, P, P, L, I, P],
@@ -153,6 +161,7 @@ DIAG_SIGNATURES: dict[str, list] = {
     "vpt_diag_occupy": [I, L, I, P, P],
 }
 _RESTYPES = {
+    "vpt_gated_norm_bwd_workspace": C.c_long,
     "vpt_lora_wgrad_workspace": C.c_long,
     "vpt_geglu_lora_partials_bytes": C.c_long,
     "vpt_gemm_workspace_bytes": C.c_long,
@@ -165,7 +174,7 @@ _RESTYPES = {
     "vpt_build_info": C.c_char_p,
 }
 # Entry points that return a value (size / count / string) rather than a status code.
-_VALUE_FNS = {"vpt_attn_bwd_queue_bytes", "vpt_grad_norm_blocks", "vpt_velocity_loss_blocks", "vpt_lora_wgrad_workspace", "vpt_geglu_lora_partials_bytes", "vpt_lora_wgrad_splits", "vpt_gemm_workspace_bytes", "vpt_linear_wgrad_workspace_bytes", "vpt_attn_fused_workspace_bytes", "vpt_cover_resize_crop_workspace", "vpt_gemm_swiglu_bwd_workspace", "vpt_rmsnorm_bwd_blocks", "vpt_layernorm_bwd_blocks", "vpt_qknorm_rope_blocks", "vpt_loss_blocks",
+_VALUE_FNS = {"vpt_gated_norm_bwd_workspace", "vpt_grad_list_piece", "vpt_grad_list_parts", "vpt_attn_bwd_queue_bytes", "vpt_grad_norm_blocks", "vpt_velocity_loss_blocks", "vpt_lora_wgrad_workspace", "vpt_geglu_lora_partials_bytes", "vpt_lora_wgrad_splits", "vpt_gemm_workspace_bytes", "vpt_linear_wgrad_workspace_bytes", "vpt_attn_fused_workspace_bytes", "vpt_cover_resize_crop_workspace", "vpt_gemm_swiglu_bwd_workspace", "vpt_rmsnorm_bwd_blocks", "vpt_layernorm_bwd_blocks", "vpt_qknorm_rope_blocks", "vpt_loss_blocks",
               "vpt_colsum_blocks", "vpt_attn_q_scale", "vpt_attn_bwd_dw_rows", "vpt_last_error_string", "vpt_abi_version", "vpt_build_info"}
 
 

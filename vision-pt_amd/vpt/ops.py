@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+from typing import NamedTuple
 
 import torch
 
@@ -1444,3 +1445,142 @@ def linear_mxfp4_dgrad(dy, w, out=None):
     dense = lambda t: t if M > 1 else t.as_strided(t.shape, (t.shape[1], 1))  # noqa: E731 (one row: any stride)
     with _on(dev):
         return linear_dgrad(dense(dy), mxfp4_dequantize(w.codes, w.scales, K), out=dense(out))
+
+
+# ----------------------------------------------------------------------------- gated norms (csrc/gated_norm.hip)
+class GatedNormGrads(NamedTuple):
+    """ops.gated_norm_bwd: dh [M, D] bf16, dx [M, D] of the stream's type; f32 gradients of the vectors, each of its vector's
+    shape, None where there is no such vector."""
+    dh: torch.Tensor
+    dx: torch.Tensor
+    dw_post: torch.Tensor | None
+    dw_pre: torch.Tensor | None
+    dgate: torch.Tensor | None
+    dscale: torch.Tensor | None
+    dshift: torch.Tensor | None
+
+
+def _gn_rows(t, name: str, dtypes, shape):
+    _rows2d(t, name, dtypes, shape)
+    _need(t.data_ptr() % 16 == 0 and (t.shape[0] <= 1 or t.stride(0) * t.element_size() % 16 == 0),
+          f"{name}: rows at multiples of 16 bytes")
+
+
+def _gn_params(name, D, M, groups, w_post, w_pre, gate, scale, shift):
+    _need(groups >= 1 and M % groups == 0, f"{name}: {M} rows do not make {groups} equal groups")
+    _need(D >= 8 and D % 8 == 0 and D <= 10240, f"{name}: D = {D}: a multiple of 8, at most 10240")
+    _need((scale is None) == (shift is None), f"{name}: scale and shift go together")
+    _need(scale is None or w_pre is not None, f"{name}: a modulation needs w_pre")
+    for v, n in ((w_post, "w_post"), (w_pre, "w_pre")):
+        if v is not None:
+            _vec1d(v, f"{name}: {n}", BF16, D)
+            _need(v.data_ptr() % 16 == 0, f"{name}: {n} at a multiple of 16 bytes")
+    for v, n in ((gate, "gate"), (scale, "scale"), (shift, "shift")):
+        if v is None:
+            continue
+        if v.dim() == 1:
+            _vec1d(v, f"{name}: {n}", BF16, D)
+            _need(v.data_ptr() % 16 == 0, f"{name}: {n} at a multiple of 16 bytes")
+        else:
+            _gn_rows(v, f"{name}: {n}", (BF16,), (groups, D))
+
+
+def _gn_vec(v):
+    """(pointer, row stride): 0 for one vector of all groups."""
+    return (None, 0) if v is None else (v.data_ptr(), 0 if v.dim() == 1 else _ld(v))
+
+
+def _gn_ptr(t):
+    return (None, 0) if t is None else (t.data_ptr(), _ld(t))
+
+
+def gated_norm_fwd(h, x, *, w_post=None, w_pre=None, gate=None, scale=None, shift=None, groups: int = 1,
+                   resid_scale: float = 1.0, eps: float = 1e-6, x_out=None, y=None):
+    """The end of a gated block and the next block's norm in one pass (vpt_gated_norm_fwd):
+
+      x_new = x + resid_scale * gate * (h * rsqrt(mean h^2 + eps) * w_post)
+      y     = x_new * rsqrt(mean x_new^2 + eps) * w_pre * (1 + scale) + shift
+
+    h [M, D] bf16 the block's output, x [M, D] the residual stream (bf16 or f32; x_new has its type and may be x: `x_out`).
+    Each vector may be left out: w_post (h enters as it is), gate, w_pre (no y), scale and shift. gate, scale and shift are
+    [D], or [groups, D] with one row for each of `groups` equal runs of rows (a sample's tokens); rows of a wider tensor do.
+    y is the norm of x_new as it is stored. D % 8 == 0, D <= 10240, rows at multiples of 16 bytes.
+    Returns (x_new, y, rstd_post, rstd_pre), the last two f32 [M] for gated_norm_bwd; None where there is no such norm."""
+    _rows2d(h, "gated_norm_fwd: h", (BF16,))
+    M, D = h.shape
+    _gn_params("gated_norm_fwd", D, M, groups, w_post, w_pre, gate, scale, shift)
+    _gn_rows(h, "gated_norm_fwd: h", (BF16,), (M, D))
+    _gn_rows(x, "gated_norm_fwd: x", (BF16, F32), (M, D))
+    if x_out is None:
+        x_out = torch.empty(M, D, dtype=x.dtype, device=x.device)
+    _gn_rows(x_out, "gated_norm_fwd: x_out", (x.dtype,), (M, D))
+    _need(y is None or w_pre is not None, "gated_norm_fwd: y needs w_pre")
+    if w_pre is not None:
+        if y is None:
+            y = torch.empty(M, D, dtype=BF16, device=x.device)
+        _gn_rows(y, "gated_norm_fwd: y", (BF16,), (M, D))
+    dev = _gpu("gated_norm_fwd", h, x, w_post, w_pre, gate, scale, shift, x_out, y)
+    rstd = torch.empty(2, M, dtype=F32, device=dev)
+    rstd_post, rstd_pre = rstd[0] if w_post is not None else None, rstd[1] if w_pre is not None else None
+    if M:
+        with _on(dev):
+            _launch("gated_norm_fwd", M * D * (2 + 2 * x.element_size() + (0 if y is None else 2)),
+                    lambda: call("vpt_gated_norm_fwd", h.data_ptr(), _ld(h), x.data_ptr(), int(x.dtype == F32), _ld(x),
+                                 _p(w_post), _p(w_pre), *_gn_vec(gate), *_gn_vec(scale), *_gn_vec(shift),
+                                 x_out.data_ptr(), _ld(x_out), *_gn_ptr(y), _p(rstd_post), _p(rstd_pre), groups,
+                                 M // groups, D, float(resid_scale), float(eps), stream()))
+    return x_out, y, rstd_post, rstd_pre
+
+
+def gated_norm_bwd(dy, dx_new, h, x_new, rstd_post, rstd_pre, *, w_post=None, w_pre=None, gate=None, scale=None,
+                   shift=None, groups: int = 1, resid_scale: float = 1.0, dh=None, dx=None) -> GatedNormGrads:
+    """The gradients of gated_norm_fwd, from dy (of y; None without w_pre) and dx_new (of x_new from what follows; None: zero,
+    only with w_pre), with h, x_new and the rstd of the forward and its vectors. The vectors' gradients are sums over rows
+    in a fixed order (the same bits every time). Without w_pre dx is dx_new itself, nothing is copied. dh may be h, and dx
+    dx_new (each element is read before it is written)."""
+    _rows2d(h, "gated_norm_bwd: h", (BF16,))
+    M, D = h.shape
+    _gn_params("gated_norm_bwd", D, M, groups, w_post, w_pre, gate, scale, shift)
+    _gn_rows(h, "gated_norm_bwd: h", (BF16,), (M, D))
+    _need(groups <= 65535, "gated_norm_bwd: at most 65535 groups")
+    kind = BF16 if w_pre is None and dx_new is None else x_new.dtype if w_pre is not None else dx_new.dtype
+    _need((dy is None) == (w_pre is None), "gated_norm_bwd: dy goes with w_pre")
+    _need(w_pre is not None or dx_new is not None, "gated_norm_bwd: dx_new without w_pre")
+    _need(w_pre is not None or dx is None, "gated_norm_bwd: without w_pre dx is dx_new")
+    if w_pre is not None:
+        _gn_rows(x_new, "gated_norm_bwd: x_new", (BF16, F32), (M, D))
+        _gn_rows(dy, "gated_norm_bwd: dy", (BF16,), (M, D))
+    else:
+        x_new = None
+    if dx_new is not None:
+        _gn_rows(dx_new, "gated_norm_bwd: dx_new", (kind,) if w_pre is not None else (BF16, F32), (M, D))
+    for r, w, n in ((rstd_post, w_post, "rstd_post"), (rstd_pre, w_pre, "rstd_pre")):
+        if w is not None:
+            _need(r is not None, f"gated_norm_bwd: {n} missing")
+            _vec1d(r, f"gated_norm_bwd: {n}", F32, M)
+    if dh is None:
+        dh = torch.empty(M, D, dtype=BF16, device=h.device)
+    _gn_rows(dh, "gated_norm_bwd: dh", (BF16,), (M, D))
+    if w_pre is None:
+        dx = dx_new
+    elif dx is None:
+        dx = torch.empty(M, D, dtype=kind, device=h.device)
+    _gn_rows(dx, "gated_norm_bwd: dx", (kind,), (M, D))
+    dev = _gpu("gated_norm_bwd", dy, dx_new, h, x_new, rstd_post if w_post is not None else None,
+               rstd_pre if w_pre is not None else None, w_post, w_pre, gate, scale, shift, dh, dx)
+    make = torch.empty if M else torch.zeros
+    grad = [None if v is None else make(v.shape, dtype=F32, device=dev) for v in (w_post, w_pre, gate, scale, shift)]
+    if M:
+        with _on(dev):
+            sums = any(g is not None for g in grad)
+            ws = torch.empty(call("vpt_gated_norm_bwd_workspace", groups, M // groups, D) if sums else 0, dtype=torch.uint8,
+                             device=dev)
+            e = h.element_size() * 2 + (dx.element_size() * 3 + 2 if w_pre is not None else dx.element_size())
+            _launch("gated_norm_bwd", M * D * e,
+                    lambda: call("vpt_gated_norm_bwd", *_gn_ptr(dy), *_gn_ptr(dx_new), h.data_ptr(), _ld(h),
+                                 _p(x_new), int(kind == F32), 0 if x_new is None else _ld(x_new), _p(rstd_post),
+                                 _p(rstd_pre), _p(w_post), _p(w_pre), *_gn_vec(gate), *_gn_vec(scale), *_gn_vec(shift),
+                                 dh.data_ptr(), _ld(dh), *(_gn_ptr(dx) if w_pre is not None else (None, 0)),
+                                 *(_p(g) for g in grad), _p(ws) if sums else None, groups, M // groups, D,
+                                 float(resid_scale), stream()))
+    return GatedNormGrads(dh, dx, *grad)

@@ -24,8 +24,10 @@ src/trainer/common.py:499-514 reads).
 
 from __future__ import annotations
 
+import bisect
 import math
 
+import numpy as np
 import torch
 
 from . import ops
@@ -129,3 +131,138 @@ class RAdamScheduleFreeFlat:
     def state_dict(self) -> dict:
         return {"param_groups": [dict(g) for g in self.param_groups], "z": self.z, "v": self.v,
                 "initialised": self._initialised}
+
+
+# ----------------------------------------------------------------------------- clipping of many gradient tensors
+_CLIP_DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
+_PIECE = np.dtype([("g", "<u8"), ("out", "<u8"), ("n", "<i4"), ("dtype", "<i4")])  # VptGradPiece
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Whether t covers numel() consecutive elements, in whatever order of its dims."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
+
+
+class GradClip:
+    """Global-norm and value clipping of a fixed list of gradient tensors, in two launches for any number of them
+    (after_backward, src/models/for_training.py:98-109; torch.nn.utils.clip_grad_norm_ and clip_grad_value_).
+
+    `grads`: dense GPU tensors of one device (bf16, f16 and f32 may be mixed; any dims, also transposed; empty ones too).
+    `out`: tensors of the same types, shapes and strides for the clipped gradients; None: in place. What is written must not
+    overlap. The handle keeps the tensors and a table of them on the device: gradients that are new tensors every step
+    (`zero_grad(set_to_none=True)`) go through clip_grad_norm_ instead. Building it copies the table to the device and
+    is not for a captured region; clip() and norm() are (their workspace is allocated per call), and may run on any stream."""
+
+    def __init__(self, grads, out=None):
+        self.grads = list(grads)
+        self.out = self.grads if out is None else list(out)
+        if len(self.out) != len(self.grads):
+            raise ValueError(f"GradClip: {len(self.out)} outputs for {len(self.grads)} gradients")
+        for g, o in zip(self.grads, self.out):
+            if not isinstance(g, torch.Tensor) or not isinstance(o, torch.Tensor):
+                raise ValueError("GradClip: tensors expected")
+            if g.layout != torch.strided or g.dtype not in _CLIP_DTYPES:
+                raise ValueError(f"GradClip: dense bf16, f16 or f32 gradients expected, got {g.dtype} {g.layout}")
+            if not _dense(g):
+                raise ValueError(f"GradClip: a gradient with gaps between its values (strides {tuple(g.stride())})")
+            if o is not g and (o.dtype != g.dtype or o.shape != g.shape or o.stride() != g.stride()):
+                raise ValueError("GradClip: an output of another type, shape or stride than its gradient")
+        written = sorted(_span(o) for o in self.out if o.numel())
+        if any(a[1] > b[0] for a, b in zip(written, written[1:])):
+            raise ValueError("GradClip: the clipped gradients overlap (the same tensor twice?)")
+        if out is not None:  # a gradient may share memory with its own output, all of it, and with no other
+            spans = sorted((*_span(o), i) for i, o in enumerate(self.out) if o.numel())
+            ends = [sp[1] for sp in spans]
+            for i, g in enumerate(self.grads):
+                if g.numel():
+                    lo, hi = _span(g)
+                    k = bisect.bisect_right(ends, lo)
+                    if k < len(spans) and spans[k][0] < hi and spans[k] != (lo, hi, i):
+                        raise ValueError("GradClip: an output overlaps another gradient, or its own in part")
+        devs = {t.device for t in self.grads + self.out}
+        if any(d.type != "cuda" for d in devs):
+            raise ValueError("GradClip: GPU tensors expected")
+        if len(devs) > 1:
+            raise ValueError("GradClip: tensors on different devices")
+        self.device = devs.pop() if devs else torch.device("cuda", torch.cuda.current_device())
+        with ops._on(self.device):
+            self._table, self._count = self._pieces()
+            self._stream = ops.stream()
+        self._parts = ops.call("vpt_grad_list_parts", self._count)
+
+    def _pieces(self):
+        piece = ops.call("vpt_grad_list_piece")
+        rows = [(g.data_ptr(), o.data_ptr(), g.numel(), _CLIP_DTYPES[g.dtype], g.element_size())
+                for g, o in zip(self.grads, self.out) if g.numel()]
+        if not rows:
+            return None, 0
+        ptr, outp, n, kind, size = (np.array(c, dtype=np.int64) for c in zip(*rows))
+        cuts = -(-n // piece)
+        first = np.cumsum(cuts) - cuts
+        at = (np.arange(int(cuts.sum())) - np.repeat(first, cuts)) * piece  # each piece's first value in its tensor
+        table = np.zeros(len(at), _PIECE)
+        table["g"] = np.repeat(ptr, cuts) + at * np.repeat(size, cuts)
+        table["out"] = np.repeat(outp, cuts) + at * np.repeat(size, cuts)
+        table["n"] = np.minimum(np.repeat(n, cuts) - at, piece)
+        table["dtype"] = np.repeat(kind, cuts)
+        return torch.from_numpy(table.view(np.uint8)).to(self.device), len(at)
+
+    def _run(self, max_norm: float, clip_value: float, count: int, want_norm: bool):
+        with ops._on(self.device):
+            st = ops.stream()
+            if st != self._stream and self._table is not None and not torch.cuda.is_current_stream_capturing():
+                self._table.record_stream(torch.cuda.current_stream())
+            table = None if self._table is None else self._table.data_ptr()
+            if not want_norm:
+                ops.call("vpt_grad_list_clip", table, count, None, 0, 0.0, clip_value, None, st)
+                return None
+            ws = torch.empty(self._parts + 1, dtype=torch.float64, device=self.device)
+            norm = ws[self._parts:].view(torch.float32)[0]
+            ops.call("vpt_grad_list_norm", table, self._count, ws.data_ptr(), st)
+            ops.call("vpt_grad_list_clip", table, count, ws.data_ptr(), self._parts, max_norm, clip_value, norm.data_ptr(), st)
+            return norm
+
+    @torch.no_grad()
+    def clip(self, max_norm: float | None = None, clip_value: float | None = None) -> torch.Tensor | None:
+        """out = clamp(min(1, max_norm / (norm + 1e-6)) * g, -clip_value, clip_value); returns the norm before it (f32, on the
+        device, not synchronised; None without max_norm). A gradient that is not finite makes the norm, and with it the
+        clipped gradients, what torch.nn.utils.clip_grad_norm_ makes of them."""
+        if max_norm is not None and not max_norm > 0:
+            raise ValueError("max_norm must be > 0")
+        if clip_value is not None and not clip_value > 0:
+            raise ValueError("clip_value must be > 0")
+        if max_norm is None and clip_value is None:
+            raise ValueError("clip: max_norm or clip_value")
+        return self._run(float(max_norm or 0.0), float(clip_value or 0.0), self._count, max_norm is not None)
+
+    @torch.no_grad()
+    def norm(self) -> torch.Tensor:
+        """The global L2 norm (f32, on the device); nothing is written."""
+        return self._run(0.0, 0.0, 0, True)
+
+
+def clip_grad_norm_(parameters, max_norm: float, clip_value: float | None = None,
+                    error_if_nonfinite: bool = False) -> torch.Tensor:
+    """torch.nn.utils.clip_grad_norm_ (L2) over parameters' .grad, then clip_grad_value_ when clip_value is given, in place.
+    Parameters without a gradient are left out; error_if_nonfinite reads the norm back before anything is scaled."""
+    params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    grads = [p.grad for p in params if p.grad is not None]
+    if not grads:
+        if not max_norm > 0:
+            raise ValueError("max_norm must be > 0")
+        return torch.tensor(0.0)
+    clipper = GradClip(grads)
+    if error_if_nonfinite and not bool(torch.isfinite(clipper.norm())):
+        raise RuntimeError("The total norm of the gradients is not finite, so it cannot be clipped.")
+    return clipper.clip(max_norm, clip_value)
