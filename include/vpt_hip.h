@@ -455,6 +455,12 @@ int vpt_mxfp4_dequantize(const void* codes, long ldc, const void* scales, long l
 int vpt_gemm_mxfp4(const void* a_codes, long lda, const void* a_scales, long ldas, const void* b_codes, long ldb,
                    const void* b_scales, long ldbs, void* C, long ldc, int M, int N, int K, const void* bias,
                    const void* resid, long ldr, int f32_out, void* stream);
+/* y[M][N] = q(x) . W^T (+ bias) (+ resid): quantize and gemm in one call (one launch for few rows). x as in quantize, W codes
+ * and scales as B of gemm. Workspace: vpt_linear_mxfp4_workspace(M, K) bytes, 16-byte aligned (0: none needed). */
+long vpt_linear_mxfp4_workspace(int M, int K);
+int vpt_linear_mxfp4(const void* x, int dtype, long ldx, const void* w_codes, long ldw, const void* w_scales, long ldws,
+                     void* y, long ldy, int M, int N, int K, const void* bias, const void* resid, long ldr, int f32_out,
+                     void* workspace, void* stream);
 /* LoRA rank-16 skinny products (lora.py:92-104 lora_down / lora_up and their weight gradients):
  * lora_proj  Y[M][16] = alpha * X[M][K] . W^T, W = down [16][K] (w_kmajor = 1) or up [K][16] (0); K % 128 == 0.
  * lora_wgrad2 both adapter gradients of one LoRA Linear: g_up [N_out][16] (+)= alpha * dY^T . dS and

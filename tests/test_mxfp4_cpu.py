@@ -92,7 +92,7 @@ def test_linear_refuses(m):
     with pytest.raises(ValueError, match="codes"):
         ops.gemm_mxfp4(*parts(4, 200), w)
     for dy, ww, msg in [(z(4, 15), w, "match"), (z(4, 16, d=torch.float32), w, "dtype"), (z(4, 24)[:, :16], w, "GPU"),
-                        (z(4, 20)[:, :16], w, "16-byte"),
+                        (z(4, 20)[:, :16], w, "16 bytes"),
                         (z(4, 12), mxfp4.MXFP4Weight(*parts(12, 64), (12, 64)), "multiples of 8"),
                         (z(4, 16), mxfp4.MXFP4Weight(*parts(16, 60), (16, 60)), "multiples of 8")]:
         with pytest.raises(ValueError, match=msg):
@@ -120,6 +120,19 @@ def test_c_abi_refuses(m):
         a = list(ok_g)
         a[i] = v
         assert lib.vpt_gemm_mxfp4(*a) == 1, (i, v)
+    ok_l = [p, 0, 256, p, 128, p, 8, p, 64, 20, 64, 256, p, p, 64, 0, p, None]
+    assert lib.vpt_linear_mxfp4_workspace(20, 256) == 20 * 136 and lib.vpt_linear_mxfp4_workspace(1, 256) == 0
+    for rows in (20, 2):  # the form with a workspace and the one without
+        for i, v in [(0, None), (0, q), (1, 3), (2, 255), (3, None), (3, p + 8), (4, 64), (4, 136), (5, None), (6, 6), (7, None),
+                     (7, q), (8, 63), (9, -1), (10, 0), (11, 0), (12, q), (13, q), (14, 63)]:
+            a = list(ok_l)
+            a[9] = rows
+            a[i] = v
+            assert lib.vpt_linear_mxfp4(*a) == 1, (rows, i, v)
+    for v in (None, p + 8):
+        a = list(ok_l)
+        a[16] = v
+        assert lib.vpt_linear_mxfp4(*a) == 1
     # nothing to do: no pointer is needed
     assert lib.vpt_mxfp4_quantize(None, 0, 256, 0, 256, None, 128, None, 8, None) == 0
     assert lib.vpt_mxfp4_dequantize(None, 128, None, 8, 0, 256, None, 256, 0, None) == 0

@@ -68,18 +68,16 @@ __device__ __forceinline__ uint32_t mx_scale(uint32_t top) {
   return be == 255u ? 255u : be > 2u ? be - 2u : 0u;
 }
 
-// Eight codes of the values f under scale byte s: e2m1 by comparisons with the seven midpoints.
+// Eight codes of the values f under scale byte s: v_cvt_scalef32_pk_fp4_f32 rounds to the nearest code, ties to even, and
+// saturates; the values are brought to the block's unit by an exact product first (s <= 252: the factor is a normal number).
 __device__ __forceinline__ uint32_t mx_codes8(const float (&f)[8], uint32_t s) {
   if (s == 255u) return 0u;
-  const float inv = __uint_as_float((254u - s) << 23);  // 2^(127 - s), s <= 252
+  const float inv = __uint_as_float((254u - s) << 23);  // 2^(127 - s)
   uint32_t out = 0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float a = fabsf(f[e]) * inv;
-    const uint32_t c = (a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) + (a >= 3.5f) + (a > 5.f);
-    out |= (c | (__float_as_uint(f[e]) >> 31 << 3)) << (4 * e);
-  }
-  return out;
+  out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(out, f[0] * inv, f[1] * inv, 1.f, 0);
+  out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(out, f[2] * inv, f[3] * inv, 1.f, 1);
+  out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(out, f[4] * inv, f[5] * inv, 1.f, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(out, f[6] * inv, f[7] * inv, 1.f, 3);
 }
 
 // One thread per 8 values: four neighbouring lanes share a block. Bound by HBM: 2 (or 4) bytes in, 17 / 32 out per value.
@@ -158,6 +156,280 @@ __device__ __forceinline__ floatx4 mx_mfma(uint4 a, uint4 b, floatx4 c, uint32_t
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_frag(a), mx_frag(b), c, 4, 4, 0, (int)sa, 0, (int)sb);
 }
 
+// ---- the tile product: TM x 128 tiles, 4 waves (2 x 2) of TM / 2 x 64, two blocks per CU -----------------------------
+// The pipeline of the bf16 256x128 ring (gemm_r2.hip), whose stages hold the same bytes here: a 3-stage LDS ring of 128-deep
+// K steps (64-byte rows of codes, 4-byte rows of scales), filled by LDS-DMA two steps ahead with counted waits. Per step and
+// wave: TM / 64 + 2 pieces of 1 KB (codes), 2 of 256 bytes (scales; for 128-row operands waves 2, 3 repeat what 0, 1 fetch, so
+// that every wave counts alike), TM / 32 + 4 fragment reads of 16 bytes and as many scale bytes per lane, TM / 8 MFMAs.
+constexpr int MXST = 3;
+template <int TM> constexpr int mx_codes_bytes() { return (TM + 128) * 64; }
+template <int TM> constexpr int mx_stage() { return mx_codes_bytes<TM>() + (TM + 128) * 4; }  // 25.5 / 17 KB
+
+__device__ __forceinline__ void glds4(const void* sbase, uint32_t voff, uint32_t lds_addr) {  // 4 bytes per lane
+  unsigned keep;
+  asm volatile("s_nop 4\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep)
+               : "v"(voff), "s"(sbase), "s"(lds_addr)
+               : "memory");
+}
+
+struct MxOffs {  // loop-invariant per-lane byte offsets of a tile's pieces
+  uint32_t a[4], b[2], as, bs;
+};
+
+template <int TM>
+__device__ __forceinline__ void mx_issue(const MxArgs& g, const MxOffs& o, int m0, int n0, int t, uint32_t smem0, int wid) {
+  const uint32_t st = smem0 + (uint32_t)(t % MXST) * mx_stage<TM>();
+  const void* ab = uniform_ptr(g.A + (long)m0 * g.lda + t * 64);
+  const void* bb = uniform_ptr(g.B + (long)n0 * g.ldb + t * 64);
+  const void* asb = uniform_ptr(g.AS + (long)m0 * g.ldas + t * 4);
+  const void* bsb = uniform_ptr(g.BS + (long)n0 * g.ldbs + t * 4);
+  const uint32_t la = __builtin_amdgcn_readfirstlane(st + wid * (TM * 16));
+  const uint32_t lb = __builtin_amdgcn_readfirstlane(st + TM * 64 + wid * 2048);
+  const uint32_t ls = st + mx_codes_bytes<TM>();
+#pragma unroll
+  for (int i = 0; i < TM / 64; ++i) glds16(ab, o.a[i], la + i * 1024);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) glds16(bb, o.b[i], lb + i * 1024);
+  glds4(asb, o.as, __builtin_amdgcn_readfirstlane(ls + (TM == 256 ? wid : wid & 1) * 256));
+  glds4(bsb, o.bs, __builtin_amdgcn_readfirstlane(ls + TM * 4 + (wid & 1) * 256));
+}
+
+// Output of 16-row fragment i: 4 KB of the wave's own LDS turn the accumulators into 8 consecutive columns of 2 rows per lane.
+// VEC: 16-byte stores (N % 8 == 0, 16-byte rows), else element by element.
+template <bool VEC, int MI>
+__device__ __forceinline__ void mx_epilogue(const MxArgs& g, const floatx4 (&acc)[MI][4], char* stg, int lane, int row0, int col0,
+                                            const float (&bias8)[8]) {
+  const int cw = lane & 7, col = col0 + cw * 8;
+  uint4 res[2][2];
+  auto load_res = [&](int i, uint4 (&r)[2]) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int row = row0 + i * 16 + p * 8 + (lane >> 3);
+      r[p] = make_uint4(0, 0, 0, 0);
+      if (VEC && g.resid && row < g.M && col < g.N)
+        r[p] = *reinterpret_cast<const uint4*>(g.resid + (long)row * g.ldr + col);
+    }
+  };
+  load_res(0, res[0]);
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    if (i + 1 < MI) load_res(i + 1, res[(i + 1) & 1]);  // one fragment ahead
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        *reinterpret_cast<float*>(stg + stg_off((lane >> 4) * 4 + r, j * 16 + (lane & 15))) = acc[i][j][r];
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): own-wave LDS writes retired
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int lr = p * 8 + (lane >> 3), row = row0 + i * 16 + lr;
+      const floatx4 x0 = *reinterpret_cast<const floatx4*>(stg + stg_off(lr, cw * 8));
+      const floatx4 x1 = *reinterpret_cast<const floatx4*>(stg + stg_off(lr, cw * 8 + 4));
+      float o[8] = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
+#pragma unroll
+      for (int q = 0; q < 8; ++q) o[q] += bias8[q];
+      if (row >= g.M) continue;
+      if (VEC) {
+        if (col >= g.N) continue;
+        if (g.resid) {
+          float rv[8];
+          unpack8(res[i & 1][p], rv);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) o[q] += rv[q];
+        }
+        if (g.f32out) {
+          float* c = reinterpret_cast<float*>(g.C) + (long)row * g.ldc + col;
+          *reinterpret_cast<floatx4*>(c) = floatx4{o[0], o[1], o[2], o[3]};
+          *reinterpret_cast<floatx4*>(c + 4) = floatx4{o[4], o[5], o[6], o[7]};
+        } else {
+          *reinterpret_cast<uint4*>(reinterpret_cast<bf16_t*>(g.C) + (long)row * g.ldc + col) = pack8(o);
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          if (col + q >= g.N) break;
+          if (g.resid) o[q] += bf2f(g.resid[(long)row * g.ldr + col + q]);
+          if (g.f32out) reinterpret_cast<float*>(g.C)[(long)row * g.ldc + col + q] = o[q];
+          else reinterpret_cast<bf16_t*>(g.C)[(long)row * g.ldc + col + q] = f2bf(o[q]);
+        }
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // this fragment's reads are done before the next one's writes
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+template <int TM, bool VEC>
+__global__ __launch_bounds__(256, 2) void mx_tile_kernel(MxArgs g) {
+  constexpr int MI = TM / 32, STG = mx_stage<TM>(), PCS = TM / 64 + 4;
+  static_assert(PCS == 8 || PCS == 6, "the counted waits below");
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, wm = wid >> 1, wn = wid & 1;
+  const int tiles_n = (g.N + 127) / 128, items = (g.M + TM - 1) / TM * tiles_n;
+  // XCD-contiguous order: the dispatcher deals block ids round-robin to the 8 XCDs, each of which runs one range of tiles
+  const int q8 = items >> 3, r8 = items & 7, xcd = blockIdx.x & 7;
+  const int tile = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (blockIdx.x >> 3);
+  const int m0 = tile / tiles_n * TM, n0 = tile % tiles_n * 128;
+  const uint32_t smem0 = (uint32_t)(uintptr_t)(VPT_LDS char*)smem;
+  MxOffs o;
+#pragma unroll
+  for (int i = 0; i < TM / 64; ++i) o.a[i] = tile_voff<true, TM, 4>(g.lda >> 1, m0, g.M, RBK, wid, lane, i);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) o.b[i] = tile_voff<true, 128, 4>(g.ldb >> 1, n0, g.N, RBK, wid, lane, i);
+  o.as = (uint32_t)(min((TM == 256 ? wid : wid & 1) * 64 + lane, g.M - 1 - m0) * (int)g.ldas);
+  o.bs = (uint32_t)(min((wid & 1) * 64 + lane, g.N - 1 - n0) * (int)g.ldbs);
+
+  float bias8[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const int c = n0 + wn * 64 + (lane & 7) * 8 + q;
+    bias8[q] = g.bias && c < g.N ? bf2f(g.bias[c]) : 0.f;
+    asm volatile("" : "+v"(bias8[q]));  // in registers before the first DMA (a later wait for it would drain the ring)
+  }
+  floatx4 acc[MI][4];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+  const int nk = g.steps;
+  mx_issue<TM>(g, o, m0, n0, 0, smem0, wid);
+  if (nk > 1) {
+    mx_issue<TM>(g, o, m0, n0, 1, smem0, wid);
+    if constexpr (PCS == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+  } else {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  }
+  __syncthreads();
+  for (int kt = 0; kt < nk; ++kt) {
+    // step kt + 2 into the stage of step kt - 1, which every wave finished reading before the last barrier
+    if (kt + 2 < nk) mx_issue<TM>(g, o, m0, n0, kt + 2, smem0, wid);
+    const char* st = smem + (kt % MXST) * STG;
+    const char* sc = st + mx_codes_bytes<TM>();
+    uint4 af[MI], bf[4];
+    uint32_t sa[MI], sb[4];
+    const int r = lane & 15, blk = lane >> 4;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int row = wn * 64 + j * 16 + r;
+      bf[j] = *reinterpret_cast<const uint4*>(st + TM * 64 + kmaj32_off(row, blk));
+      sb[j] = *reinterpret_cast<const uint8_t*>(sc + TM * 4 + row * 4 + blk);
+    }
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int row = wm * (TM / 2) + i * 16 + r;
+      af[i] = *reinterpret_cast<const uint4*>(st + kmaj32_off(row, blk));
+      sa[i] = *reinterpret_cast<const uint8_t*>(sc + row * 4 + blk);
+    }
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = mx_mfma(af[i], bf[j], acc[i][j], sa[i], sb[j]);
+    __builtin_amdgcn_s_setprio(0);
+    if (kt + 1 < nk) {
+      // this wave's pieces of step kt + 1 landed (step kt + 2's younger ones may still fly), then every wave's
+      if (kt + 2 < nk) {
+        if constexpr (PCS == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
+      __syncthreads();
+    }
+  }
+  // staging: this wave's 4 KB of the stage of step nk - 3 (or an unused one), which nobody reads or fills any more
+  mx_epilogue<VEC, MI>(g, acc, smem + (nk % MXST) * STG + wid * 4096, lane, m0 + wm * (TM / 2), n0 + wn * 64, bias8);
+}
+
+// ---- few rows: 16 MI rows x 16 columns per block, its 4 waves share the steps along K --------------------------------
+// With few rows the product is a pass over W: each wave takes every fourth 128-deep step, its 16 rows of W straight from
+// memory into registers (four steps' loads in flight), and the four partial sums meet in LDS in a fixed order. FUSE: the block
+// quantises its rows of x itself, into LDS (M <= 16; the same codes as mx_quantize_kernel), and saves a launch.
+struct MxX {
+  const void* x; long ldx;
+  int K;
+};
+constexpr int kMxSkinnyLoads = 4;
+
+template <int MI, int FUSE, bool XVEC>  // FUSE: 0 no, else 1 + the type of x
+__global__ __launch_bounds__(256) void mx_skinny_kernel(MxArgs g, MxX x) {
+  __shared__ float red[4][16 * MI][17];
+  extern __shared__ __attribute__((aligned(16))) char smem[];  // FUSE: codes [M][64 steps + 16], scales [M][4 steps]
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (16 * MI);
+  const int pitch = 64 * g.steps + 16;
+  char* lscale = smem + (long)g.M * pitch;
+  if (FUSE) {
+    const int nch = 16 * g.steps, total = g.M * nch;
+    for (int idx = tid; idx < total; idx += 256) {  // total % 16 == 0: the four lanes of a block stay together
+      const int row = idx / nch, c = idx - row * nch;
+      float f[8];
+      mx_load8<FUSE - 1, XVEC>(x.x, (long)row * x.ldx + c * 8, c * 8, x.K, f);
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
+      top = max(top, dpp_xor1(top));
+      top = max(top, dpp_xor2(top));
+      const uint32_t sc = mx_scale(top);
+      *reinterpret_cast<uint32_t*>(smem + row * pitch + c * 4) = mx_codes8(f, sc);
+      if ((c & 3) == 0) lscale[row * 4 * g.steps + (c >> 2)] = (char)sc;
+    }
+    __syncthreads();
+  }
+  const int r = lane & 15, blk = lane >> 4;
+  const long wrow = min(n0 + r, g.N - 1);  // rows past the edge: the last one (its results are not stored)
+  const uint8_t* wb = g.B + wrow * g.ldb + blk * 16;
+  const uint8_t* ws = g.BS + wrow * g.ldbs + blk;
+  const uint8_t* ab[MI];
+  const uint8_t* as[MI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const long row = min(m0 + i * 16 + r, g.M - 1);
+    ab[i] = FUSE ? (const uint8_t*)smem + row * pitch + blk * 16 : g.A + row * g.lda + blk * 16;
+    as[i] = FUSE ? (const uint8_t*)lscale + row * 4 * g.steps + blk : g.AS + row * g.ldas + blk;
+  }
+  floatx4 acc[MI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i) acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  for (int t0 = wid; t0 < g.steps; t0 += 4 * kMxSkinnyLoads) {
+    uint4 bf[kMxSkinnyLoads];
+    uint32_t sb[kMxSkinnyLoads];
+#pragma unroll
+    for (int u = 0; u < kMxSkinnyLoads; ++u) {
+      const int t = min(t0 + 4 * u, g.steps - 1);  // past the end: loaded, not used
+      bf[u] = *reinterpret_cast<const uint4*>(wb + (long)t * 64);
+      sb[u] = ws[(long)t * 4];
+    }
+#pragma unroll
+    for (int u = 0; u < kMxSkinnyLoads; ++u) {
+      const int t = t0 + 4 * u;  // wave-uniform
+      if (t >= g.steps) break;
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+        acc[i] = mx_mfma(*reinterpret_cast<const uint4*>(ab[i] + (long)t * 64), bf[u], acc[i], as[i][(long)t * 4], sb[u]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) red[wid][i * 16 + blk * 4 + q][r] = acc[i][q];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int lr = i * 16 + (tid >> 4), c = tid & 15, m = m0 + lr, n = n0 + c;
+    if (m >= g.M || n >= g.N) continue;
+    float v = (red[0][lr][c] + red[1][lr][c]) + (red[2][lr][c] + red[3][lr][c]);
+    if (g.bias) v += bf2f(g.bias[n]);
+    if (g.resid) v += bf2f(g.resid[(long)m * g.ldr + n]);
+    if (g.f32out) reinterpret_cast<float*>(g.C)[(long)m * g.ldc + n] = v;
+    else reinterpret_cast<bf16_t*>(g.C)[(long)m * g.ldc + n] = f2bf(v);
+  }
+}
+
 // 128 x 128 tile, 4 waves of 64 x 64, one 128-deep step at a time through LDS.
 __global__ __launch_bounds__(256) void mx_gemm_kernel(MxArgs g) {
   __shared__ __attribute__((aligned(16))) char as[128 * 64], bs[128 * 64];
@@ -225,6 +497,71 @@ void mx_quantize_launch(const void* x, long ldx, long rows, unsigned nch, int K,
   const unsigned total = (unsigned)(rows * nch);
   hipLaunchKernelGGL((mx_quantize_kernel<T, VEC>), dim3((total + 255u) / 256u), dim3(256), 0, s, x, ldx, total, nch, K,
                      codes, ldc, scales, lds);
+}
+
+
+// W, the output, bias and residual of a product.
+int mx_check_product(const void* b_codes, long ldb, const void* b_scales, long ldbs, const void* C, long ldc, int M, int N, int K,
+                     const void* bias, const void* resid, long ldr, int f32_out) {
+  const long steps = (K + 127) / 128;
+  VPT_CHECK_ARG(b_codes && b_scales && C, "mxfp4 product: null pointer");
+  VPT_CHECK_ARG(ldb >= 64 * steps && ldb % 16 == 0 && aligned(b_codes, 16),
+                "mxfp4 product: code rows of 64 ceil(K / 128) bytes at multiples of 16 bytes");
+  VPT_CHECK_ARG(ldbs >= 4 * steps && ldbs % 4 == 0 && aligned(b_scales, 4),
+                "mxfp4 product: scale rows of 4 ceil(K / 128) bytes at multiples of 4 bytes");
+  VPT_CHECK_ARG((ldc >= N || M == 1) && aligned(C, f32_out ? 4 : 2), "mxfp4 product: output rows of N values, aligned to their type");
+  VPT_CHECK_ARG((!bias || aligned(bias, 2)) && (!resid || (aligned(resid, 2) && (ldr >= N || M == 1))),
+                "mxfp4 product: bf16 bias and residual, rows of N values");
+  VPT_CHECK_ARG(((M + 127L) / 128) * ((N + 127L) / 128) < (1L << 31), "mxfp4 product: too many tiles");
+  return VPT_OK;
+}
+
+constexpr int kMxSkinnyRows = 64;
+
+template <int MI>
+void mx_skinny_launch(const MxArgs& g, hipStream_t s) {
+  hipLaunchKernelGGL((mx_skinny_kernel<MI, 0, false>), dim3((g.N + 15) / 16, (g.M + 16 * MI - 1) / (16 * MI)), dim3(256), 0, s, g,
+                     MxX{nullptr, 0, 0});
+}
+
+// The product of checked arguments.
+void mx_product(const MxArgs& g, hipStream_t st) {
+  const long tiles = ((g.M + 127L) / 128) * ((g.N + 127L) / 128);
+  if (g.M <= kMxSkinnyRows) {
+    if (g.M <= 16) mx_skinny_launch<1>(g, st);
+    else if (g.M <= 32) mx_skinny_launch<2>(g, st);
+    else mx_skinny_launch<4>(g, st);
+    return;
+  }
+  // the tile kernels keep 32-bit offsets within a tile of at most 256 rows
+  const long es = g.f32out ? 4 : 2, far = 1L << 22;
+  if (g.lda >= far || g.ldb >= far || g.ldas >= far || g.ldbs >= far) {
+    hipLaunchKernelGGL(mx_gemm_kernel, dim3((unsigned)tiles), dim3(256), 0, st, g);
+    return;
+  }
+  const bool vec = g.N % 8 == 0 && aligned(g.C, 16) && g.ldc * es % 16 == 0 &&
+                   (!g.resid || (aligned(g.resid, 16) && g.ldr % 8 == 0));
+  const long tiles256 = ((g.M + 255L) / 256) * ((g.N + 127L) / 128);
+  if (tiles256 >= 512) {
+    if (vec) hipLaunchKernelGGL((mx_tile_kernel<256, true>), dim3((unsigned)tiles256), dim3(256), MXST * mx_stage<256>(), st, g);
+    else hipLaunchKernelGGL((mx_tile_kernel<256, false>), dim3((unsigned)tiles256), dim3(256), MXST * mx_stage<256>(), st, g);
+  } else {
+    if (vec) hipLaunchKernelGGL((mx_tile_kernel<128, true>), dim3((unsigned)tiles), dim3(256), MXST * mx_stage<128>(), st, g);
+    else hipLaunchKernelGGL((mx_tile_kernel<128, false>), dim3((unsigned)tiles), dim3(256), MXST * mx_stage<128>(), st, g);
+  }
+}
+
+// LDS of the fused form, 0 where it is not taken.
+size_t mx_fused_lds(long M, int K) {
+  const long steps = (K + 127) / 128, bytes = M * (68 * steps + 16);
+  return M <= 16 && bytes <= 48 * 1024 ? (size_t)bytes : 0;
+}
+
+template <int T>
+void mx_fused_launch(const MxArgs& g, const MxX& x, bool vec, size_t lds, hipStream_t s) {
+  const dim3 grid((g.N + 15) / 16, 1);
+  if (vec) hipLaunchKernelGGL((mx_skinny_kernel<1, T + 1, true>), grid, dim3(256), lds, s, g, x);
+  else hipLaunchKernelGGL((mx_skinny_kernel<1, T + 1, false>), grid, dim3(256), lds, s, g, x);
 }
 
 }  // namespace
@@ -301,22 +638,55 @@ extern "C" int vpt_gemm_mxfp4(const void* a_codes, long lda, const void* a_scale
                               const void* bias, const void* resid, long ldr, int f32_out, void* stream) {
   VPT_CHECK_ARG(M >= 0 && N > 0 && K > 0 && K <= (1 << 30), "vpt_gemm_mxfp4: M >= 0, N > 0, 0 < K <= 2^30");
   if (M == 0) return VPT_OK;
-  VPT_CHECK_ARG(a_codes && a_scales && b_codes && b_scales && C, "vpt_gemm_mxfp4: null pointer");
   const int steps = (K + 127) / 128;
-  VPT_CHECK_ARG(lda >= 64L * steps && lda % 16 == 0 && aligned(a_codes, 16) && ldb >= 64L * steps && ldb % 16 == 0 &&
-                    aligned(b_codes, 16),
+  VPT_CHECK_ARG(a_codes && a_scales, "vpt_gemm_mxfp4: null pointer");
+  VPT_CHECK_ARG(lda >= 64L * steps && lda % 16 == 0 && aligned(a_codes, 16),
                 "vpt_gemm_mxfp4: code rows of 64 ceil(K / 128) bytes at multiples of 16 bytes");
-  VPT_CHECK_ARG(ldas >= 4L * steps && ldas % 4 == 0 && aligned(a_scales, 4) && ldbs >= 4L * steps && ldbs % 4 == 0 &&
-                    aligned(b_scales, 4),
+  VPT_CHECK_ARG(ldas >= 4L * steps && ldas % 4 == 0 && aligned(a_scales, 4),
                 "vpt_gemm_mxfp4: scale rows of 4 ceil(K / 128) bytes at multiples of 4 bytes");
-  VPT_CHECK_ARG((ldc >= N || M == 1) && aligned(C, f32_out ? 4 : 2), "vpt_gemm_mxfp4: ldc >= N, C aligned to its type");
-  VPT_CHECK_ARG((!bias || aligned(bias, 2)) && (!resid || (aligned(resid, 2) && (ldr >= N || M == 1))),
-                "vpt_gemm_mxfp4: bf16 bias and residual, ldr >= N");
-  const long tiles = ((M + 127L) / 128) * ((N + 127L) / 128);
-  VPT_CHECK_ARG(tiles < (1L << 31), "vpt_gemm_mxfp4: too many tiles");
+  const int rc = mx_check_product(b_codes, ldb, b_scales, ldbs, C, ldc, M, N, K, bias, resid, ldr, f32_out);
+  if (rc) return rc;
   const MxArgs g{(const uint8_t*)a_codes, lda, (const uint8_t*)a_scales, ldas, (const uint8_t*)b_codes, ldb,
                  (const uint8_t*)b_scales, ldbs, C, ldc, (const bf16_t*)bias, (const bf16_t*)resid, ldr, M, N, steps, f32_out};
-  hipLaunchKernelGGL(mx_gemm_kernel, dim3((unsigned)tiles), dim3(256), 0, (hipStream_t)stream, g);
+  mx_product(g, (hipStream_t)stream);
+  VPT_LAUNCH_CHECK();
+  return VPT_OK;
+}
+
+extern "C" long vpt_linear_mxfp4_workspace(int M, int K) {
+  if (M <= 0 || K <= 0 || K > (1 << 30) || mx_fused_lds(M, K)) return 0;
+  return M * 68L * ((K + 127) / 128);
+}
+
+extern "C" int vpt_linear_mxfp4(const void* x, int dtype, long ldx, const void* w_codes, long ldw, const void* w_scales,
+                                long ldws, void* y, long ldy, int M, int N, int K, const void* bias, const void* resid, long ldr,
+                                int f32_out, void* workspace, void* stream) {
+  VPT_CHECK_ARG(dtype >= MX_BF16 && dtype <= MX_F16, "vpt_linear_mxfp4: dtype 0 bf16, 1 f32, 2 f16");
+  VPT_CHECK_ARG(M >= 0 && N > 0 && K > 0 && K <= (1 << 30), "vpt_linear_mxfp4: M >= 0, N > 0, 0 < K <= 2^30");
+  if (M == 0) return VPT_OK;
+  const int es = dtype == MX_F32 ? 4 : 2;
+  VPT_CHECK_ARG(x && aligned(x, es) && (ldx >= K || M == 1), "vpt_linear_mxfp4: x aligned to its type, ldx >= K");
+  const long steps = (K + 127) / 128;
+  const int rc = mx_check_product(w_codes, ldw, w_scales, ldws, y, ldy, M, N, K, bias, resid, ldr, f32_out);
+  if (rc) return rc;
+  const size_t lds = mx_fused_lds(M, K);
+  uint8_t* codes = (uint8_t*)workspace;
+  uint8_t* scales = codes + M * 64L * steps;
+  if (!lds) {
+    VPT_CHECK_ARG(workspace && aligned(workspace, 16), "vpt_linear_mxfp4: workspace of vpt_linear_mxfp4_workspace bytes");
+    const int qrc = vpt_mxfp4_quantize(x, dtype, ldx, M, K, codes, 64 * steps, scales, 4 * steps, stream);
+    if (qrc) return qrc;
+    return vpt_gemm_mxfp4(codes, 64 * steps, scales, 4 * steps, w_codes, ldw, w_scales, ldws, y, ldy, M, N, K, bias, resid, ldr,
+                          f32_out, stream);
+  }
+  const MxArgs g{nullptr, 0, nullptr, 0, (const uint8_t*)w_codes, ldw, (const uint8_t*)w_scales, ldws, y, ldy,
+                 (const bf16_t*)bias, (const bf16_t*)resid, ldr, M, N, (int)steps, f32_out};
+  const MxX xx{x, ldx, K};
+  const bool vec = K % 8 == 0 && aligned(x, 16) && (M == 1 || ldx * es % 16 == 0);
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == MX_BF16) mx_fused_launch<MX_BF16>(g, xx, vec, lds, st);
+  else if (dtype == MX_F32) mx_fused_launch<MX_F32>(g, xx, vec, lds, st);
+  else mx_fused_launch<MX_F16>(g, xx, vec, lds, st);
   VPT_LAUNCH_CHECK();
   return VPT_OK;
 }

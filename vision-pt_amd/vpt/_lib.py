@@ -121,6 +121,8 @@ SIGNATURES: dict[str, list] = {
     "vpt_mxfp4_quantize": [P, I, L, L, I, P, L, P, L, P],
     "vpt_mxfp4_dequantize": [P, L, P, L, L, I, P, L, I, P],
     "vpt_gemm_mxfp4": [P, L, P, L, P, L, P, L, P, L, I, I, I, P, P, L, I, P],
+    "vpt_linear_mxfp4_workspace": [I, I],
+    "vpt_linear_mxfp4": [P, I, L, P, L, P, L, P, L, I, I, I, P, P, L, I, P, P],
     "vpt_add_bf16": [P, P, L, P, P],
     "vpt_flow_noise": [P, P, L, I, F, I, U64, P, P, P, P],
     "vpt_velocity_loss_blocks": [],
@@ -162,6 +164,7 @@ DIAG_SIGNATURES: dict[str, list] = {
 }
 _RESTYPES = {
     "vpt_gated_norm_bwd_workspace": C.c_long,
+    "vpt_linear_mxfp4_workspace": C.c_long,
     "vpt_lora_wgrad_workspace": C.c_long,
     "vpt_geglu_lora_partials_bytes": C.c_long,
     "vpt_gemm_workspace_bytes": C.c_long,
@@ -174,7 +177,7 @@ _RESTYPES = {
     "vpt_build_info": C.c_char_p,
 }
 # Entry points that return a value (size / count / string) rather than a status code.
-_VALUE_FNS = {"vpt_gated_norm_bwd_workspace", "vpt_grad_list_piece", "vpt_grad_list_parts", "vpt_attn_bwd_queue_bytes", "vpt_grad_norm_blocks", "vpt_velocity_loss_blocks", "vpt_lora_wgrad_workspace", "vpt_geglu_lora_partials_bytes", "vpt_lora_wgrad_splits", "vpt_gemm_workspace_bytes", "vpt_linear_wgrad_workspace_bytes", "vpt_attn_fused_workspace_bytes", "vpt_cover_resize_crop_workspace", "vpt_gemm_swiglu_bwd_workspace", "vpt_rmsnorm_bwd_blocks", "vpt_layernorm_bwd_blocks", "vpt_qknorm_rope_blocks", "vpt_loss_blocks",
+_VALUE_FNS = {"vpt_linear_mxfp4_workspace", "vpt_gated_norm_bwd_workspace", "vpt_grad_list_piece", "vpt_grad_list_parts", "vpt_attn_bwd_queue_bytes", "vpt_grad_norm_blocks", "vpt_velocity_loss_blocks", "vpt_lora_wgrad_workspace", "vpt_geglu_lora_partials_bytes", "vpt_lora_wgrad_splits", "vpt_gemm_workspace_bytes", "vpt_linear_wgrad_workspace_bytes", "vpt_attn_fused_workspace_bytes", "vpt_cover_resize_crop_workspace", "vpt_gemm_swiglu_bwd_workspace", "vpt_rmsnorm_bwd_blocks", "vpt_layernorm_bwd_blocks", "vpt_qknorm_rope_blocks", "vpt_loss_blocks",
               "vpt_colsum_blocks", "vpt_attn_q_scale", "vpt_attn_bwd_dw_rows", "vpt_last_error_string", "vpt_abi_version", "vpt_build_info"}
 
 

@@ -1269,15 +1269,16 @@ def cover_resize_crop(img_u8, in_h, in_w, scaled_h, scaled_w, top, left, out_h, 
     return out
 
 
-# ----------------------------------------------------------------------------- MXFP4 (csrc/mxfp4.hip)
-_MX_DTYPES = {BF16: 0, F32: 1, torch.float16: 2}
+# ----------------------------------------------------------------------------- checks of the calls below
+# A call on a few tokens is bound by the host, so a check that holds costs one expression and no message is put together.
+def _on(index: int):
+    """The device of a call's tensors as the current one (a launch goes to the current device)."""
+    return contextlib.nullcontext() if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
-def _on(dev: torch.device):
-    """The device of a call's tensors as the current one (a launch goes to the current device's stream)."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
+def _raw_stream(index: int) -> int:
+    """The current stream of device `index` (what torch.cuda.current_stream(index).cuda_stream holds, without the object)."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _need(cond: bool, msg: str):
@@ -1285,25 +1286,38 @@ def _need(cond: bool, msg: str):
         raise ValueError(msg)
 
 
-def _gpu(name: str, *ts):
-    """All of ts (None: left out) on one GPU; returns that device. Called after the checks of shapes and types."""
-    dev = None
+def _gpu(name: str, *ts) -> int:
+    """All of ts (None: left out) on one GPU; returns its index. Called after the checks of shapes and types."""
+    dev = ts[0].get_device()
     for t in ts:
-        if t is None:
-            continue
-        _need(t.is_cuda, f"{name}: GPU tensors expected")
-        _need(dev is None or t.device == dev, f"{name}: tensors on different devices")
-        dev = t.device
+        if t is not None and t.get_device() != dev or dev < 0:
+            raise ValueError(f"{name}: GPU tensors expected" if dev < 0 or t.get_device() < 0
+                             else f"{name}: tensors on different devices")
     return dev
 
 
-def _rows2d(t, name: str, dtypes, shape=None):
-    """A [rows, cols] tensor of one of dtypes whose rows are contiguous and do not overlap."""
-    _need(t.dtype in dtypes, f"{name}: dtype {t.dtype}, expected one of {[str(d) for d in dtypes]}")
+def _rows2d(t, fn: str, arg: str, dtypes, shape=None, align: int = 1):
+    """A [rows, cols] tensor of one of dtypes whose rows are contiguous, do not overlap and start at multiples of `align`
+    bytes."""
+    sh = t.shape
+    if (t.dtype in dtypes and (len(sh) == 2 if shape is None else sh == shape) and t.is_contiguous()
+            and (align == 1 or t.data_ptr() % align == 0 and (sh[0] <= 1 or sh[1] * t.element_size() % align == 0))):
+        return
+    _need(t.dtype in dtypes, f"{fn}: {arg}: dtype {t.dtype}, expected one of {[str(d) for d in dtypes]}")
     _need(t.dim() == 2 and (shape is None or tuple(t.shape) == tuple(shape)),
-          f"{name}: shape {tuple(t.shape)}, expected {'[rows, cols]' if shape is None else tuple(shape)}")
-    _need(t.shape[1] <= 1 or t.stride(1) == 1, f"{name}: the last dim must be contiguous")
-    _need(t.shape[0] <= 1 or t.stride(0) >= t.shape[1], f"{name}: rows must not overlap (row stride {t.stride(0)})")
+          f"{fn}: {arg}: shape {tuple(t.shape)}, expected {'[rows, cols]' if shape is None else tuple(shape)}")
+    _need(t.shape[1] <= 1 or t.stride(1) == 1, f"{fn}: {arg}: the last dim must be contiguous")
+    _need(t.shape[0] <= 1 or t.stride(0) >= t.shape[1], f"{fn}: {arg}: rows must not overlap (row stride {t.stride(0)})")
+    _need(t.data_ptr() % align == 0 and (t.shape[0] <= 1 or t.stride(0) * t.element_size() % align == 0),
+          f"{fn}: {arg}: rows at multiples of {align} bytes")
+
+
+def _vec1d(t, fn: str, arg: str, dtype, n: int, align: int = 1):
+    sh = t.shape
+    if not (t.dtype == dtype and len(sh) == 1 and sh[0] == n and (n <= 1 or t.stride(0) == 1)):
+        raise ValueError(f"{fn}: {arg}: a contiguous {dtype} [{n}] tensor expected, got {t.dtype} {tuple(t.shape)}")
+    if align > 1 and t.data_ptr() % align:
+        raise ValueError(f"{fn}: {arg} at a multiple of {align} bytes")
 
 
 def _ld(t) -> int:
@@ -1311,9 +1325,14 @@ def _ld(t) -> int:
     return t.stride(0) if t.shape[0] > 1 else max(1, t.shape[1])
 
 
-def _vec1d(t, name: str, dtype, n: int):
-    _need(t.dtype == dtype and tuple(t.shape) == (n,) and (n <= 1 or t.stride(0) == 1),
-          f"{name}: a contiguous {dtype} [{n}] tensor expected, got {t.dtype} {tuple(t.shape)}")
+def _ptr_ld(t):
+    return (None, 0) if t is None else (t.data_ptr(), _ld(t))
+
+
+# ----------------------------------------------------------------------------- MXFP4 (csrc/mxfp4.hip)
+_MX_DTYPES = {BF16: 0, F32: 1, torch.float16: 2}
+_U8 = (torch.uint8,)
+_MX_OUT = (BF16, F32)
 
 
 def mxfp4_shapes(rows: int, K: int) -> tuple[tuple[int, int], tuple[int, int]]:
@@ -1322,14 +1341,10 @@ def mxfp4_shapes(rows: int, K: int) -> tuple[tuple[int, int], tuple[int, int]]:
     return (rows, 64 * steps), (rows, 4 * steps)
 
 
-def _mx_parts(codes, scales, rows, K, name: str):
-    cs, ss = mxfp4_shapes(rows, K)
-    _rows2d(codes, f"{name}: codes", (torch.uint8,), cs)
-    _rows2d(scales, f"{name}: scales", (torch.uint8,), ss)
-    _need(codes.data_ptr() % 16 == 0 and (rows <= 1 or codes.stride(0) % 16 == 0),
-          f"{name}: code rows at multiples of 16 bytes")
-    _need(scales.data_ptr() % 4 == 0 and (rows <= 1 or scales.stride(0) % 4 == 0),
-          f"{name}: scale rows at multiples of 4 bytes")
+def _mx_parts(codes, scales, rows, K, fn: str):
+    steps = (K + 127) // 128
+    _rows2d(codes, fn, "codes", _U8, (rows, 64 * steps), 16)
+    _rows2d(scales, fn, "scales", _U8, (rows, 4 * steps), 4)
 
 
 def mxfp4_quantize(x, codes=None, scales=None):
@@ -1338,23 +1353,24 @@ def mxfp4_quantize(x, codes=None, scales=None):
     A block of 32 consecutive values of a row shares the scale 2^(s - 127), s = max(floor(log2 max|x|) + 125, 0); a code is
     x / 2^(s - 127) rounded to the nearest of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6}, ties to the even code, saturated at 6. A block
     with an infinity or a NaN reads back as NaN. Rows are padded with zeros to 128 values (include/vpt_hip.h)."""
-    _rows2d(x, "mxfp4_quantize: x", tuple(_MX_DTYPES))
+    _rows2d(x, "mxfp4_quantize", "x", _MX_DTYPES)
     M, K = x.shape
     _need(K >= 1, "mxfp4_quantize: K >= 1")
     cs, ss = mxfp4_shapes(M, K)
+    given = codes is not None or scales is not None
     if codes is None:
         codes = torch.empty(cs, dtype=torch.uint8, device=x.device)
     if scales is None:
         scales = torch.empty(ss, dtype=torch.uint8, device=x.device)
-    _mx_parts(codes, scales, M, K, "mxfp4_quantize")
+    if given:
+        _mx_parts(codes, scales, M, K, "mxfp4_quantize")
     dev = _gpu("mxfp4_quantize", x, codes, scales)
     if M == 0:
         return codes, scales
-    es = x.element_size()
     with _on(dev):
-        _launch("mxfp4_quantize", M * K * (es + 17 / 32),
-                lambda: call("vpt_mxfp4_quantize", x.data_ptr(), _MX_DTYPES[x.dtype], _ld(x), M, K,
-                             codes.data_ptr(), _ld(codes), scales.data_ptr(), _ld(scales), stream()))
+        _launch("mxfp4_quantize", M * K * (x.element_size() + 17 / 32),
+                lambda: call("vpt_mxfp4_quantize", x.data_ptr(), _MX_DTYPES[x.dtype], _ld(x), M, K, codes.data_ptr(),
+                             _ld(codes), scales.data_ptr(), _ld(scales), _raw_stream(dev)))
     return codes, scales
 
 
@@ -1364,28 +1380,30 @@ def mxfp4_dequantize(codes, scales, K: int, out=None, dtype=BF16):
     M = codes.shape[0]
     _mx_parts(codes, scales, M, K, "mxfp4_dequantize")
     if out is None:
-        _need(dtype in (BF16, F32), "mxfp4_dequantize: dtype bf16 or f32")
+        _need(dtype in _MX_OUT, "mxfp4_dequantize: dtype bf16 or f32")
         out = torch.empty(M, K, dtype=dtype, device=codes.device)
-    _rows2d(out, "mxfp4_dequantize: out", (BF16, F32), (M, K))
+    else:
+        _rows2d(out, "mxfp4_dequantize", "out", _MX_OUT, (M, K))
     dev = _gpu("mxfp4_dequantize", codes, scales, out)
     if M == 0:
         return out
     with _on(dev):
         _launch("mxfp4_dequantize", M * K * (out.element_size() + 17 / 32),
-                lambda: call("vpt_mxfp4_dequantize", codes.data_ptr(), _ld(codes), scales.data_ptr(),
-                             _ld(scales), M, K, out.data_ptr(), _ld(out), int(out.dtype == F32), stream()))
+                lambda: call("vpt_mxfp4_dequantize", codes.data_ptr(), _ld(codes), scales.data_ptr(), _ld(scales), M, K,
+                             out.data_ptr(), _ld(out), int(out.dtype == F32), _raw_stream(dev)))
     return out
 
 
-def _mx_out(name, M, N, dev, bias, resid, out, out_dtype):
+def _mx_out(fn, M, N, dev, bias, resid, out, out_dtype):
     if out is None:
-        _need(out_dtype in (BF16, F32), f"{name}: out bf16 or f32")
+        _need(out_dtype in _MX_OUT, f"{fn}: out bf16 or f32")
         out = torch.empty(M, N, dtype=out_dtype, device=dev)
-    _rows2d(out, f"{name}: out", (BF16, F32), (M, N))
+    else:
+        _rows2d(out, fn, "out", _MX_OUT, (M, N))
     if bias is not None:
-        _vec1d(bias, f"{name}: bias", BF16, N)
+        _vec1d(bias, fn, "bias", BF16, N)
     if resid is not None:
-        _rows2d(resid, f"{name}: resid", (BF16,), (M, N))
+        _rows2d(resid, fn, "resid", (BF16,), (M, N))
     return out
 
 
@@ -1400,29 +1418,35 @@ def gemm_mxfp4(a_codes, a_scales, w, out=None, *, bias=None, resid=None, out_dty
     dev = _gpu("gemm_mxfp4", a_codes, a_scales, w.codes, w.scales, out, bias, resid)
     if M == 0:
         return out
-
-    def run():
-        call("vpt_gemm_mxfp4", a_codes.data_ptr(), _ld(a_codes), a_scales.data_ptr(), _ld(a_scales),
-             w.codes.data_ptr(), _ld(w.codes), w.scales.data_ptr(), _ld(w.scales), out.data_ptr(),
-             _ld(out), M, N, K, _p(bias), _p(resid), 0 if resid is None else _ld(resid),
-             int(out.dtype == F32), stream())
     with _on(dev):
-        _launch("gemm_mxfp4", 2.0 * M * N * K, run)
+        _launch("gemm_mxfp4", 2.0 * M * N * K,
+                lambda: call("vpt_gemm_mxfp4", a_codes.data_ptr(), _ld(a_codes), a_scales.data_ptr(), _ld(a_scales),
+                             w.codes.data_ptr(), _ld(w.codes), w.scales.data_ptr(), _ld(w.scales), out.data_ptr(),
+                             _ld(out), M, N, K, _p(bias), *_ptr_ld(resid), int(out.dtype == F32), _raw_stream(dev)))
     return out
 
 
 def linear_mxfp4(x, w, bias=None, resid=None, out=None, out_dtype=BF16):
     """y = q(x) . W^T (+ bias) (+ resid): nn.Linear on an MXFP4 weight with its input quantised to MXFP4 on the way
-    (x [M, K] bf16, f16 or f32; w a vpt.mxfp4.MXFP4Weight [N, K]). y is bf16 or f32."""
-    _rows2d(x, "linear_mxfp4: x", tuple(_MX_DTYPES))
-    _need(x.shape[1] == w.shape[1], f"linear_mxfp4: x {tuple(x.shape)} does not match W {w.shape}")
-    out = _mx_out("linear_mxfp4", x.shape[0], w.shape[0], x.device, bias, resid, out, out_dtype)
+    (x [M, K] bf16, f16 or f32; w a vpt.mxfp4.MXFP4Weight [N, K]): mxfp4_quantize and gemm_mxfp4, in one launch for a few rows.
+    y is bf16 or f32; `out` may be `resid` itself."""
+    _rows2d(x, "linear_mxfp4", "x", _MX_DTYPES)
+    M, K = x.shape
+    N = w.shape[0]
+    if K != w.shape[1]:
+        raise ValueError(f"linear_mxfp4: x {tuple(x.shape)} does not match W {w.shape}")
+    out = _mx_out("linear_mxfp4", M, N, x.device, bias, resid, out, out_dtype)
     dev = _gpu("linear_mxfp4", x, w.codes, w.scales, out, bias, resid)
-    if x.shape[0] == 0:
+    if M == 0:
         return out
+    n = call("vpt_linear_mxfp4_workspace", M, K)
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
     with _on(dev):
-        codes, scales = mxfp4_quantize(x)
-        return gemm_mxfp4(codes, scales, w, out, bias=bias, resid=resid)
+        _launch("linear_mxfp4", 2.0 * M * N * K,
+                lambda: call("vpt_linear_mxfp4", x.data_ptr(), _MX_DTYPES[x.dtype], _ld(x), w.codes.data_ptr(),
+                             _ld(w.codes), w.scales.data_ptr(), _ld(w.scales), out.data_ptr(), _ld(out), M, N, K, _p(bias),
+                             *_ptr_ld(resid), int(out.dtype == F32), _p(ws), _raw_stream(dev)))
+    return out
 
 
 def linear_mxfp4_dgrad(dy, w, out=None):
@@ -1430,21 +1454,24 @@ def linear_mxfp4_dgrad(dy, w, out=None):
     [M, K] bf16). W is dequantised to bf16 (exact) and goes through the bf16 GEMM, whose rows start at multiples of 16
     bytes: N % 8 == 0 and K % 8 == 0, and dy and out with such rows."""
     N, K = w.shape
-    _rows2d(dy, "linear_mxfp4_dgrad: dy", (BF16,))
-    _need(dy.shape[1] == N, f"linear_mxfp4_dgrad: dy {tuple(dy.shape)} does not match W {w.shape}")
-    _need(N % 8 == 0 and K % 8 == 0, f"linear_mxfp4_dgrad: N and K multiples of 8, W {w.shape}")
     M = dy.shape[0]
+    _rows2d(dy, "linear_mxfp4_dgrad", "dy", (BF16,))
+    if dy.shape[1] != N:
+        raise ValueError(f"linear_mxfp4_dgrad: dy {tuple(dy.shape)} does not match W {w.shape}")
+    if N % 8 or K % 8:
+        raise ValueError(f"linear_mxfp4_dgrad: N and K multiples of 8, W {w.shape}")
+    _rows2d(dy, "linear_mxfp4_dgrad", "dy", (BF16,), None, 16)
     if out is None:
         out = torch.empty(M, K, dtype=BF16, device=dy.device)
-    _rows2d(out, "linear_mxfp4_dgrad: out", (BF16,), (M, K))
-    for t, n in ((dy, "dy"), (out, "out")):
-        _need(t.data_ptr() % 16 == 0 and (M <= 1 or t.stride(0) % 8 == 0), f"linear_mxfp4_dgrad: {n}: 16-byte rows")
+    else:
+        _rows2d(out, "linear_mxfp4_dgrad", "out", (BF16,), (M, K), 16)
     dev = _gpu("linear_mxfp4_dgrad", dy, w.codes, w.scales, out)
     if M == 0:
         return out
     dense = lambda t: t if M > 1 else t.as_strided(t.shape, (t.shape[1], 1))  # noqa: E731 (one row: any stride)
     with _on(dev):
-        return linear_dgrad(dense(dy), mxfp4_dequantize(w.codes, w.scales, K), out=dense(out))
+        linear_dgrad(dense(dy), mxfp4_dequantize(w.codes, w.scales, K), out=dense(out))
+    return out
 
 
 # ----------------------------------------------------------------------------- gated norms (csrc/gated_norm.hip)
@@ -1460,38 +1487,33 @@ class GatedNormGrads(NamedTuple):
     dshift: torch.Tensor | None
 
 
-def _gn_rows(t, name: str, dtypes, shape):
-    _rows2d(t, name, dtypes, shape)
-    _need(t.data_ptr() % 16 == 0 and (t.shape[0] <= 1 or t.stride(0) * t.element_size() % 16 == 0),
-          f"{name}: rows at multiples of 16 bytes")
+_BF16 = (BF16,)
 
 
-def _gn_params(name, D, M, groups, w_post, w_pre, gate, scale, shift):
-    _need(groups >= 1 and M % groups == 0, f"{name}: {M} rows do not make {groups} equal groups")
-    _need(D >= 8 and D % 8 == 0 and D <= 10240, f"{name}: D = {D}: a multiple of 8, at most 10240")
-    _need((scale is None) == (shift is None), f"{name}: scale and shift go together")
-    _need(scale is None or w_pre is not None, f"{name}: a modulation needs w_pre")
-    for v, n in ((w_post, "w_post"), (w_pre, "w_pre")):
-        if v is not None:
-            _vec1d(v, f"{name}: {n}", BF16, D)
-            _need(v.data_ptr() % 16 == 0, f"{name}: {n} at a multiple of 16 bytes")
+def _gn_params(fn, D, M, groups, w_post, w_pre, gate, scale, shift):
+    if not (groups >= 1 and M % groups == 0):
+        raise ValueError(f"{fn}: {M} rows do not make {groups} equal groups")
+    if not (D >= 8 and D % 8 == 0 and D <= 10240):
+        raise ValueError(f"{fn}: D = {D}: a multiple of 8, at most 10240")
+    if (scale is None) != (shift is None):
+        raise ValueError(f"{fn}: scale and shift go together")
+    if scale is not None and w_pre is None:
+        raise ValueError(f"{fn}: a modulation needs w_pre")
+    if w_post is not None:
+        _vec1d(w_post, fn, "w_post", BF16, D, 16)
+    if w_pre is not None:
+        _vec1d(w_pre, fn, "w_pre", BF16, D, 16)
     for v, n in ((gate, "gate"), (scale, "scale"), (shift, "shift")):
-        if v is None:
-            continue
-        if v.dim() == 1:
-            _vec1d(v, f"{name}: {n}", BF16, D)
-            _need(v.data_ptr() % 16 == 0, f"{name}: {n} at a multiple of 16 bytes")
-        else:
-            _gn_rows(v, f"{name}: {n}", (BF16,), (groups, D))
+        if v is not None:
+            if v.dim() == 1:
+                _vec1d(v, fn, n, BF16, D, 16)
+            else:
+                _rows2d(v, fn, n, _BF16, (groups, D), 16)
 
 
 def _gn_vec(v):
     """(pointer, row stride): 0 for one vector of all groups."""
     return (None, 0) if v is None else (v.data_ptr(), 0 if v.dim() == 1 else _ld(v))
-
-
-def _gn_ptr(t):
-    return (None, 0) if t is None else (t.data_ptr(), _ld(t))
 
 
 def gated_norm_fwd(h, x, *, w_post=None, w_pre=None, gate=None, scale=None, shift=None, groups: int = 1,
@@ -1506,29 +1528,30 @@ def gated_norm_fwd(h, x, *, w_post=None, w_pre=None, gate=None, scale=None, shif
     [D], or [groups, D] with one row for each of `groups` equal runs of rows (a sample's tokens); rows of a wider tensor do.
     y is the norm of x_new as it is stored. D % 8 == 0, D <= 10240, rows at multiples of 16 bytes.
     Returns (x_new, y, rstd_post, rstd_pre), the last two f32 [M] for gated_norm_bwd; None where there is no such norm."""
-    _rows2d(h, "gated_norm_fwd: h", (BF16,))
+    _rows2d(h, "gated_norm_fwd", "h", _BF16)
     M, D = h.shape
     _gn_params("gated_norm_fwd", D, M, groups, w_post, w_pre, gate, scale, shift)
-    _gn_rows(h, "gated_norm_fwd: h", (BF16,), (M, D))
-    _gn_rows(x, "gated_norm_fwd: x", (BF16, F32), (M, D))
+    _rows2d(h, "gated_norm_fwd", "h", _BF16, (M, D), 16)
+    _rows2d(x, "gated_norm_fwd", "x", _MX_OUT, (M, D), 16)
     if x_out is None:
         x_out = torch.empty(M, D, dtype=x.dtype, device=x.device)
-    _gn_rows(x_out, "gated_norm_fwd: x_out", (x.dtype,), (M, D))
-    _need(y is None or w_pre is not None, "gated_norm_fwd: y needs w_pre")
-    if w_pre is not None:
-        if y is None:
-            y = torch.empty(M, D, dtype=BF16, device=x.device)
-        _gn_rows(y, "gated_norm_fwd: y", (BF16,), (M, D))
+    else:
+        _rows2d(x_out, "gated_norm_fwd", "x_out", (x.dtype,), (M, D), 16)
+    if y is not None:
+        _need(w_pre is not None, "gated_norm_fwd: y needs w_pre")
+        _rows2d(y, "gated_norm_fwd", "y", _BF16, (M, D), 16)
+    elif w_pre is not None:
+        y = torch.empty(M, D, dtype=BF16, device=x.device)
     dev = _gpu("gated_norm_fwd", h, x, w_post, w_pre, gate, scale, shift, x_out, y)
-    rstd = torch.empty(2, M, dtype=F32, device=dev)
-    rstd_post, rstd_pre = rstd[0] if w_post is not None else None, rstd[1] if w_pre is not None else None
+    rstd_post = None if w_post is None else torch.empty(M, dtype=F32, device=x.device)
+    rstd_pre = None if w_pre is None else torch.empty(M, dtype=F32, device=x.device)
     if M:
         with _on(dev):
             _launch("gated_norm_fwd", M * D * (2 + 2 * x.element_size() + (0 if y is None else 2)),
                     lambda: call("vpt_gated_norm_fwd", h.data_ptr(), _ld(h), x.data_ptr(), int(x.dtype == F32), _ld(x),
                                  _p(w_post), _p(w_pre), *_gn_vec(gate), *_gn_vec(scale), *_gn_vec(shift),
-                                 x_out.data_ptr(), _ld(x_out), *_gn_ptr(y), _p(rstd_post), _p(rstd_pre), groups,
-                                 M // groups, D, float(resid_scale), float(eps), stream()))
+                                 x_out.data_ptr(), _ld(x_out), *_ptr_ld(y), _p(rstd_post), _p(rstd_pre), groups,
+                                 M // groups, D, float(resid_scale), float(eps), _raw_stream(dev)))
     return x_out, y, rstd_post, rstd_pre
 
 
@@ -1538,49 +1561,53 @@ def gated_norm_bwd(dy, dx_new, h, x_new, rstd_post, rstd_pre, *, w_post=None, w_
     only with w_pre), with h, x_new and the rstd of the forward and its vectors. The vectors' gradients are sums over rows
     in a fixed order (the same bits every time). Without w_pre dx is dx_new itself, nothing is copied. dh may be h, and dx
     dx_new (each element is read before it is written)."""
-    _rows2d(h, "gated_norm_bwd: h", (BF16,))
+    fn = "gated_norm_bwd"
+    _rows2d(h, fn, "h", _BF16)
     M, D = h.shape
-    _gn_params("gated_norm_bwd", D, M, groups, w_post, w_pre, gate, scale, shift)
-    _gn_rows(h, "gated_norm_bwd: h", (BF16,), (M, D))
+    _gn_params(fn, D, M, groups, w_post, w_pre, gate, scale, shift)
+    _rows2d(h, fn, "h", _BF16, (M, D), 16)
     _need(groups <= 65535, "gated_norm_bwd: at most 65535 groups")
-    kind = BF16 if w_pre is None and dx_new is None else x_new.dtype if w_pre is not None else dx_new.dtype
     _need((dy is None) == (w_pre is None), "gated_norm_bwd: dy goes with w_pre")
-    _need(w_pre is not None or dx_new is not None, "gated_norm_bwd: dx_new without w_pre")
-    _need(w_pre is not None or dx is None, "gated_norm_bwd: without w_pre dx is dx_new")
     if w_pre is not None:
-        _gn_rows(x_new, "gated_norm_bwd: x_new", (BF16, F32), (M, D))
-        _gn_rows(dy, "gated_norm_bwd: dy", (BF16,), (M, D))
+        _rows2d(x_new, fn, "x_new", _MX_OUT, (M, D), 16)
+        _rows2d(dy, fn, "dy", _BF16, (M, D), 16)
+        _need(rstd_pre is not None, "gated_norm_bwd: rstd_pre missing")
+        _vec1d(rstd_pre, fn, "rstd_pre", F32, M)
+        kind = x_new.dtype
+        if dx_new is not None:
+            _rows2d(dx_new, fn, "dx_new", (kind,), (M, D), 16)
+        if dx is None:
+            dx = torch.empty(M, D, dtype=kind, device=h.device)
+        else:
+            _rows2d(dx, fn, "dx", (kind,), (M, D), 16)
     else:
-        x_new = None
-    if dx_new is not None:
-        _gn_rows(dx_new, "gated_norm_bwd: dx_new", (kind,) if w_pre is not None else (BF16, F32), (M, D))
-    for r, w, n in ((rstd_post, w_post, "rstd_post"), (rstd_pre, w_pre, "rstd_pre")):
-        if w is not None:
-            _need(r is not None, f"gated_norm_bwd: {n} missing")
-            _vec1d(r, f"gated_norm_bwd: {n}", F32, M)
+        _need(dx_new is not None, "gated_norm_bwd: dx_new without w_pre")
+        _need(dx is None, "gated_norm_bwd: without w_pre dx is dx_new")
+        _rows2d(dx_new, fn, "dx_new", _MX_OUT, (M, D), 16)
+        dx, kind, x_new, rstd_pre = dx_new, dx_new.dtype, None, None
+    if w_post is not None:
+        _need(rstd_post is not None, "gated_norm_bwd: rstd_post missing")
+        _vec1d(rstd_post, fn, "rstd_post", F32, M)
+    else:
+        rstd_post = None
     if dh is None:
         dh = torch.empty(M, D, dtype=BF16, device=h.device)
-    _gn_rows(dh, "gated_norm_bwd: dh", (BF16,), (M, D))
-    if w_pre is None:
-        dx = dx_new
-    elif dx is None:
-        dx = torch.empty(M, D, dtype=kind, device=h.device)
-    _gn_rows(dx, "gated_norm_bwd: dx", (kind,), (M, D))
-    dev = _gpu("gated_norm_bwd", dy, dx_new, h, x_new, rstd_post if w_post is not None else None,
-               rstd_pre if w_pre is not None else None, w_post, w_pre, gate, scale, shift, dh, dx)
+    else:
+        _rows2d(dh, fn, "dh", _BF16, (M, D), 16)
+    dev = _gpu("gated_norm_bwd", h, dy, dx_new, x_new, rstd_post, rstd_pre, w_post, w_pre, gate, scale, shift, dh, dx)
     make = torch.empty if M else torch.zeros
-    grad = [None if v is None else make(v.shape, dtype=F32, device=dev) for v in (w_post, w_pre, gate, scale, shift)]
+    grad = [None if v is None else make(v.shape, dtype=F32, device=h.device) for v in (w_post, w_pre, gate, scale, shift)]
     if M:
         with _on(dev):
             sums = any(g is not None for g in grad)
-            ws = torch.empty(call("vpt_gated_norm_bwd_workspace", groups, M // groups, D) if sums else 0, dtype=torch.uint8,
-                             device=dev)
+            ws = torch.empty(call("vpt_gated_norm_bwd_workspace", groups, M // groups, D), dtype=torch.uint8,
+                             device=h.device) if sums else None
             e = h.element_size() * 2 + (dx.element_size() * 3 + 2 if w_pre is not None else dx.element_size())
             _launch("gated_norm_bwd", M * D * e,
-                    lambda: call("vpt_gated_norm_bwd", *_gn_ptr(dy), *_gn_ptr(dx_new), h.data_ptr(), _ld(h),
+                    lambda: call("vpt_gated_norm_bwd", *_ptr_ld(dy), *_ptr_ld(dx_new), h.data_ptr(), _ld(h),
                                  _p(x_new), int(kind == F32), 0 if x_new is None else _ld(x_new), _p(rstd_post),
                                  _p(rstd_pre), _p(w_post), _p(w_pre), *_gn_vec(gate), *_gn_vec(scale), *_gn_vec(shift),
-                                 dh.data_ptr(), _ld(dh), *(_gn_ptr(dx) if w_pre is not None else (None, 0)),
-                                 *(_p(g) for g in grad), _p(ws) if sums else None, groups, M // groups, D,
-                                 float(resid_scale), stream()))
+                                 dh.data_ptr(), _ld(dh), *(_ptr_ld(dx) if w_pre is not None else (None, 0)),
+                                 *(_p(g) for g in grad), _p(ws), groups, M // groups, D,
+                                 float(resid_scale), _raw_stream(dev)))
     return GatedNormGrads(dh, dx, *grad)

@@ -196,9 +196,9 @@ class GradClip:
         if len(devs) > 1:
             raise ValueError("GradClip: tensors on different devices")
         self.device = devs.pop() if devs else torch.device("cuda", torch.cuda.current_device())
-        with ops._on(self.device):
+        with ops._on(self.device.index):
             self._table, self._count = self._pieces()
-            self._stream = ops.stream()
+            self._stream = ops._raw_stream(self.device.index)
         self._parts = ops.call("vpt_grad_list_parts", self._count)
 
     def _pieces(self):
@@ -219,8 +219,8 @@ class GradClip:
         return torch.from_numpy(table.view(np.uint8)).to(self.device), len(at)
 
     def _run(self, max_norm: float, clip_value: float, count: int, want_norm: bool):
-        with ops._on(self.device):
-            st = ops.stream()
+        with ops._on(self.device.index):
+            st = ops._raw_stream(self.device.index)
             if st != self._stream and self._table is not None and not torch.cuda.is_current_stream_capturing():
                 self._table.record_stream(torch.cuda.current_stream())
             table = None if self._table is None else self._table.data_ptr()
