@@ -13,6 +13,8 @@
 // lane, 64-byte rows per step), at four times the values per byte.
 #include "gemm_common.h"
 
+#include <type_traits>
+
 namespace {
 
 using namespace vptg;
@@ -158,19 +160,21 @@ __device__ __forceinline__ floatx4 mx_mfma(uint4 a, uint4 b, floatx4 c, uint32_t
 
 // ---- the tile product: TM x 128 tiles, 4 waves (2 x 2) of TM / 2 x 64, two blocks per CU -----------------------------
 // The pipeline of the bf16 256x128 ring (gemm_r2.hip), whose stages hold the same bytes here: a 3-stage LDS ring of 128-deep
-// K steps (64-byte rows of codes, 4-byte rows of scales), filled by LDS-DMA two steps ahead with counted waits. Per step and
-// wave: TM / 64 + 2 pieces of 1 KB (codes), 2 of 256 bytes (scales; for 128-row operands waves 2, 3 repeat what 0, 1 fetch, so
-// that every wave counts alike), TM / 32 + 4 fragment reads of 16 bytes and as many scale bytes per lane, TM / 8 MFMAs.
+// K steps (64-byte rows of codes) filled by LDS-DMA two steps ahead with counted waits. Per step and wave TM / 64 + 2 pieces of
+// 1 KB, TM / 32 + 4 fragment reads of 16 bytes and TM / 8 MFMAs.
+// Scales: 16 bytes per row, those of 4 steps, in one piece of 16 bytes per lane (rows of 4 bytes per step cost as many cache
+// accesses as the codes: 1.39x the time at 33360 x 4096 x 3840). They have one buffer: a wave takes its rows' bytes of all 4
+// steps into registers at the first of them, and the next 4 steps' piece is fetched from the second on.
+// The product is taken transposed, W's fragment first, so that a lane holds 4 consecutive columns of one output row; W's rows
+// lie in LDS in an order (mx_wrow) that makes the columns of two fragments neighbours: 16-byte stores from registers.
 constexpr int MXST = 3;
-template <int TM> constexpr int mx_codes_bytes() { return (TM + 128) * 64; }
-template <int TM> constexpr int mx_stage() { return mx_codes_bytes<TM>() + (TM + 128) * 4; }  // 25.5 / 17 KB
+template <int TM> constexpr int mx_stage() { return (TM + 128) * 64; }               // 24 / 16 KB
+template <int TM> constexpr int mx_lds() { return MXST * mx_stage<TM>() + (TM + 128) * 16; }  // 78 / 52 KB
 
-__device__ __forceinline__ void glds4(const void* sbase, uint32_t voff, uint32_t lds_addr) {  // 4 bytes per lane
-  unsigned keep;
-  asm volatile("s_nop 4\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b32 m0, %0"
-               : "=&s"(keep)
-               : "v"(voff), "s"(sbase), "s"(lds_addr)
-               : "memory");
+// Position p of a wave's 64 rows of W in LDS holds row mx_wrow(p): fragment j = p >> 4, row i = p & 15 of the MFMA operand;
+// output rows 4 g + e of fragments 2 q, 2 q + 1 become columns 32 q + 8 g + 0 .. 7.
+__device__ __forceinline__ int mx_wrow(int p) {
+  return (p >> 5) * 32 + ((p >> 2) & 3) * 8 + ((p >> 4) & 1) * 4 + (p & 3);
 }
 
 struct MxOffs {  // loop-invariant per-lane byte offsets of a tile's pieces
@@ -182,62 +186,54 @@ __device__ __forceinline__ void mx_issue(const MxArgs& g, const MxOffs& o, int m
   const uint32_t st = smem0 + (uint32_t)(t % MXST) * mx_stage<TM>();
   const void* ab = uniform_ptr(g.A + (long)m0 * g.lda + t * 64);
   const void* bb = uniform_ptr(g.B + (long)n0 * g.ldb + t * 64);
-  const void* asb = uniform_ptr(g.AS + (long)m0 * g.ldas + t * 4);
-  const void* bsb = uniform_ptr(g.BS + (long)n0 * g.ldbs + t * 4);
   const uint32_t la = __builtin_amdgcn_readfirstlane(st + wid * (TM * 16));
   const uint32_t lb = __builtin_amdgcn_readfirstlane(st + TM * 64 + wid * 2048);
-  const uint32_t ls = st + mx_codes_bytes<TM>();
-#pragma unroll
-  for (int i = 0; i < TM / 64; ++i) glds16(ab, o.a[i], la + i * 1024);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) glds16(bb, o.b[i], lb + i * 1024);
-  glds4(asb, o.as, __builtin_amdgcn_readfirstlane(ls + (TM == 256 ? wid : wid & 1) * 256));
-  glds4(bsb, o.bs, __builtin_amdgcn_readfirstlane(ls + TM * 4 + (wid & 1) * 256));
+  if constexpr (TM == 256) {
+    glds_step(ab, bb, o.a[0], o.a[1], o.b[0], o.b[1], la, la + 1024, lb, lb + 1024);
+    glds16(ab, o.a[2], la + 2048);
+    glds16(ab, o.a[3], la + 3072);
+  } else {
+    glds_step(ab, bb, o.a[0], o.a[1], o.b[0], o.b[1], la, la + 1024, lb, lb + 1024);
+  }
 }
 
-// Output of 16-row fragment i: 4 KB of the wave's own LDS turn the accumulators into 8 consecutive columns of 2 rows per lane.
-// VEC: 16-byte stores (N % 8 == 0, 16-byte rows), else element by element.
+// The scale bytes from `at` on, 16 per row (waves 2, 3 repeat what 0, 1 fetch of a 128-row operand: every wave counts alike).
+template <int TM>
+__device__ __forceinline__ void mx_issue_scales(const MxArgs& g, const MxOffs& o, int m0, int n0, int at, uint32_t smem0, int wid) {
+  const uint32_t ls = smem0 + MXST * mx_stage<TM>();
+  glds16(uniform_ptr(g.AS + (long)m0 * g.ldas + at), o.as,
+         __builtin_amdgcn_readfirstlane(ls + (TM == 256 ? wid : wid & 1) * 1024));
+  glds16(uniform_ptr(g.BS + (long)n0 * g.ldbs + at), o.bs, __builtin_amdgcn_readfirstlane(ls + TM * 16 + (wid & 1) * 1024));
+}
+
+template <int S>
+__device__ __forceinline__ floatx4 mx_mfma_at(uint4 a, uint4 b, floatx4 c, uint32_t sa, uint32_t sb) {  // scale byte S
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_frag(a), mx_frag(b), c, 4, 4, S, (int)sa, S, (int)sb);
+}
+
+// acc[i][j][e]: row 16 i + (lane & 15), column 32 (j >> 1) + 8 (lane >> 4) + 4 (j & 1) + e of the wave's tile. VEC: 16-byte
+// accesses (N % 8 == 0, 16-byte rows), else element by element.
 template <bool VEC, int MI>
-__device__ __forceinline__ void mx_epilogue(const MxArgs& g, const floatx4 (&acc)[MI][4], char* stg, int lane, int row0, int col0,
-                                            const float (&bias8)[8]) {
-  const int cw = lane & 7, col = col0 + cw * 8;
-  uint4 res[2][2];
-  auto load_res = [&](int i, uint4 (&r)[2]) {
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const int row = row0 + i * 16 + p * 8 + (lane >> 3);
-      r[p] = make_uint4(0, 0, 0, 0);
-      if (VEC && g.resid && row < g.M && col < g.N)
-        r[p] = *reinterpret_cast<const uint4*>(g.resid + (long)row * g.ldr + col);
-    }
-  };
-  load_res(0, res[0]);
+__device__ __forceinline__ void mx_epilogue(const MxArgs& g, const floatx4 (&acc)[MI][4], int lane, int row0, int col0,
+                                            const float (&bias)[2][8]) {
+  const int c0 = col0 + (lane >> 4) * 8;
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
-    if (i + 1 < MI) load_res(i + 1, res[(i + 1) & 1]);  // one fragment ahead
+    const int row = row0 + i * 16 + (lane & 15);
+    if (row >= g.M) continue;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int q = 0; q < 2; ++q) {
+      const int col = c0 + q * 32;
+      float o[8];
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        *reinterpret_cast<float*>(stg + stg_off((lane >> 4) * 4 + r, j * 16 + (lane & 15))) = acc[i][j][r];
-    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): own-wave LDS writes retired
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const int lr = p * 8 + (lane >> 3), row = row0 + i * 16 + lr;
-      const floatx4 x0 = *reinterpret_cast<const floatx4*>(stg + stg_off(lr, cw * 8));
-      const floatx4 x1 = *reinterpret_cast<const floatx4*>(stg + stg_off(lr, cw * 8 + 4));
-      float o[8] = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
-#pragma unroll
-      for (int q = 0; q < 8; ++q) o[q] += bias8[q];
-      if (row >= g.M) continue;
+      for (int e = 0; e < 8; ++e) o[e] = acc[i][2 * q + (e >> 2)][e & 3] + bias[q][e];
       if (VEC) {
         if (col >= g.N) continue;
         if (g.resid) {
           float rv[8];
-          unpack8(res[i & 1][p], rv);
+          unpack8(*reinterpret_cast<const uint4*>(g.resid + (long)row * g.ldr + col), rv);
 #pragma unroll
-          for (int q = 0; q < 8; ++q) o[q] += rv[q];
+          for (int e = 0; e < 8; ++e) o[e] += rv[e];
         }
         if (g.f32out) {
           float* c = reinterpret_cast<float*>(g.C) + (long)row * g.ldc + col;
@@ -248,23 +244,21 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& g, const floatx4 (&acc
         }
       } else {
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          if (col + q >= g.N) break;
-          if (g.resid) o[q] += bf2f(g.resid[(long)row * g.ldr + col + q]);
-          if (g.f32out) reinterpret_cast<float*>(g.C)[(long)row * g.ldc + col + q] = o[q];
-          else reinterpret_cast<bf16_t*>(g.C)[(long)row * g.ldc + col + q] = f2bf(o[q]);
+        for (int e = 0; e < 8; ++e) {
+          if (col + e >= g.N) break;
+          if (g.resid) o[e] += bf2f(g.resid[(long)row * g.ldr + col + e]);
+          if (g.f32out) reinterpret_cast<float*>(g.C)[(long)row * g.ldc + col + e] = o[e];
+          else reinterpret_cast<bf16_t*>(g.C)[(long)row * g.ldc + col + e] = f2bf(o[e]);
         }
       }
     }
-    __builtin_amdgcn_s_waitcnt(0xc07f);  // this fragment's reads are done before the next one's writes
-    __builtin_amdgcn_wave_barrier();
   }
 }
 
 template <int TM, bool VEC>
 __global__ __launch_bounds__(256, 2) void mx_tile_kernel(MxArgs g) {
-  constexpr int MI = TM / 32, STG = mx_stage<TM>(), PCS = TM / 64 + 4;
-  static_assert(PCS == 8 || PCS == 6, "the counted waits below");
+  constexpr int MI = TM / 32, STG = mx_stage<TM>(), PCS = TM / 64 + 2;
+  static_assert(PCS == 6 || PCS == 4, "the counted waits below");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, wm = wid >> 1, wn = wid & 1;
   const int tiles_n = (g.N + 127) / 128, items = (g.M + TM - 1) / TM * tiles_n;
@@ -273,20 +267,41 @@ __global__ __launch_bounds__(256, 2) void mx_tile_kernel(MxArgs g) {
   const int tile = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (blockIdx.x >> 3);
   const int m0 = tile / tiles_n * TM, n0 = tile % tiles_n * 128;
   const uint32_t smem0 = (uint32_t)(uintptr_t)(VPT_LDS char*)smem;
-  MxOffs o;
+  const int nk = g.steps, r = lane & 15, blk = lane >> 4;
+  MxOffs o;  // rows past the edge: the last one (its results are not stored)
 #pragma unroll
   for (int i = 0; i < TM / 64; ++i) o.a[i] = tile_voff<true, TM, 4>(g.lda >> 1, m0, g.M, RBK, wid, lane, i);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) o.b[i] = tile_voff<true, 128, 4>(g.ldb >> 1, n0, g.N, RBK, wid, lane, i);
+  for (int i = 0; i < 2; ++i) {
+    const int p = (wid * 2 + i) * 16 + (lane >> 2), row = (p & 64) | mx_wrow(p & 63);
+    o.b[i] = (uint32_t)(min(row, g.N - 1 - n0) * (int)g.ldb + ((lane & 3) ^ (((p >> 2) & 1) << 1)) * 16);
+  }
   o.as = (uint32_t)(min((TM == 256 ? wid : wid & 1) * 64 + lane, g.M - 1 - m0) * (int)g.ldas);
-  o.bs = (uint32_t)(min((wid & 1) * 64 + lane, g.N - 1 - n0) * (int)g.ldbs);
+  o.bs = (uint32_t)(min((wid & 1) * 64 + mx_wrow(lane), g.N - 1 - n0) * (int)g.ldbs);
 
-  float bias8[8];
+  float bias[2][8];
 #pragma unroll
-  for (int q = 0; q < 8; ++q) {
-    const int c = n0 + wn * 64 + (lane & 7) * 8 + q;
-    bias8[q] = g.bias && c < g.N ? bf2f(g.bias[c]) : 0.f;
-    asm volatile("" : "+v"(bias8[q]));  // in registers before the first DMA (a later wait for it would drain the ring)
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int c = n0 + wn * 64 + q * 32 + blk * 8 + e;
+      bias[q][e] = g.bias && c < g.N ? bf2f(g.bias[c]) : 0.f;
+      asm volatile("" : "+v"(bias[q][e]));  // in registers before the first DMA (a later wait for it would drain the ring)
+    }
+  uint32_t sa[MI], sb[4];
+#pragma unroll
+  for (int i = 0; i < MI; ++i) sa[i] = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sb[j] = 0;
+  if (nk < 4) {  // no 16 bytes of scales in a row: straight into registers
+    for (int t = 0; t < nk; ++t) {
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+        sa[i] |= (uint32_t)g.AS[(long)min(m0 + wm * (TM / 2) + i * 16 + r, g.M - 1) * g.ldas + t * 4 + blk] << (8 * t);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        sb[j] |= (uint32_t)g.BS[(long)min(n0 + wn * 64 + mx_wrow(j * 16 + r), g.N - 1) * g.ldbs + t * 4 + blk] << (8 * t);
+    }
   }
   floatx4 acc[MI][4];
 #pragma unroll
@@ -294,55 +309,78 @@ __global__ __launch_bounds__(256, 2) void mx_tile_kernel(MxArgs g) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
 
-  const int nk = g.steps;
+  if (nk >= 4) mx_issue_scales<TM>(g, o, m0, n0, 0, smem0, wid);
   mx_issue<TM>(g, o, m0, n0, 0, smem0, wid);
   if (nk > 1) {
     mx_issue<TM>(g, o, m0, n0, 1, smem0, wid);
-    if constexpr (PCS == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-    else asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+    if constexpr (PCS == 6) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
   } else {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
   __syncthreads();
-  for (int kt = 0; kt < nk; ++kt) {
+
+  // Step kt = 4 c + S.
+  auto step = [&](int kt, auto S_) {
+    constexpr int S = decltype(S_)::value;
+    // the next 4 steps' scales: the buffer was read at step 4 c; a last group of fewer than 4 ends with the row
+    const bool fetch = S == 1 && kt + 3 < nk;
+    if (fetch) mx_issue_scales<TM>(g, o, m0, n0, min(4 * (kt + 3), 4 * nk - 16), smem0, wid);
     // step kt + 2 into the stage of step kt - 1, which every wave finished reading before the last barrier
     if (kt + 2 < nk) mx_issue<TM>(g, o, m0, n0, kt + 2, smem0, wid);
     const char* st = smem + (kt % MXST) * STG;
-    const char* sc = st + mx_codes_bytes<TM>();
+    if (S == 0 && nk >= 4) {
+      const char* sc = smem + MXST * STG + blk;
+      const int rem = nk - kt, first = rem < 4 ? 4 - rem : 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint8_t* p = reinterpret_cast<const uint8_t*>(sc + TM * 16 + (wn * 64 + j * 16 + r) * 16);
+        sb[j] = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sb[j] |= (uint32_t)p[min(first + e, 3) * 4] << (8 * e);
+      }
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        const uint8_t* p = reinterpret_cast<const uint8_t*>(sc + (wm * (TM / 2) + i * 16 + r) * 16);
+        sa[i] = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sa[i] |= (uint32_t)p[min(first + e, 3) * 4] << (8 * e);
+      }
+    }
     uint4 af[MI], bf[4];
-    uint32_t sa[MI], sb[4];
-    const int r = lane & 15, blk = lane >> 4;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int row = wn * 64 + j * 16 + r;
-      bf[j] = *reinterpret_cast<const uint4*>(st + TM * 64 + kmaj32_off(row, blk));
-      sb[j] = *reinterpret_cast<const uint8_t*>(sc + TM * 4 + row * 4 + blk);
-    }
+    for (int j = 0; j < 4; ++j)
+      bf[j] = *reinterpret_cast<const uint4*>(st + TM * 64 + kmaj32_off(wn * 64 + j * 16 + r, blk));
 #pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      const int row = wm * (TM / 2) + i * 16 + r;
-      af[i] = *reinterpret_cast<const uint4*>(st + kmaj32_off(row, blk));
-      sa[i] = *reinterpret_cast<const uint8_t*>(sc + row * 4 + blk);
-    }
+    for (int i = 0; i < MI; ++i) af[i] = *reinterpret_cast<const uint4*>(st + kmaj32_off(wm * (TM / 2) + i * 16 + r, blk));
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = mx_mfma(af[i], bf[j], acc[i][j], sa[i], sb[j]);
+      for (int j = 0; j < 4; ++j) acc[i][j] = mx_mfma_at<S>(bf[j], af[i], acc[i][j], sb[j], sa[i]);
     __builtin_amdgcn_s_setprio(0);
     if (kt + 1 < nk) {
-      // this wave's pieces of step kt + 1 landed (step kt + 2's younger ones may still fly), then every wave's
-      if (kt + 2 < nk) {
-        if constexpr (PCS == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+      // this wave's pieces of step kt + 1 landed (those of step kt + 2, and scales issued with them, may still fly), then
+      // every wave's
+      if (kt + 2 >= nk) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      } else if (fetch) {
+        if constexpr (PCS == 6) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
         else asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
       } else {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if constexpr (PCS == 6) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
       }
       __syncthreads();
     }
+  };
+  for (int kt = 0; kt < nk; kt += 4) {
+    step(kt, std::integral_constant<int, 0>{});
+    if (kt + 1 < nk) step(kt + 1, std::integral_constant<int, 1>{});
+    if (kt + 2 < nk) step(kt + 2, std::integral_constant<int, 2>{});
+    if (kt + 3 < nk) step(kt + 3, std::integral_constant<int, 3>{});
   }
-  // staging: this wave's 4 KB of the stage of step nk - 3 (or an unused one), which nobody reads or fills any more
-  mx_epilogue<VEC, MI>(g, acc, smem + (nk % MXST) * STG + wid * 4096, lane, m0 + wm * (TM / 2), n0 + wn * 64, bias8);
+  mx_epilogue<VEC, MI>(g, acc, lane, m0 + wm * (TM / 2), n0 + wn * 64, bias);
 }
 
 // ---- few rows: 16 MI rows x 16 columns per block, its 4 waves share the steps along K --------------------------------
@@ -543,11 +581,11 @@ void mx_product(const MxArgs& g, hipStream_t st) {
                    (!g.resid || (aligned(g.resid, 16) && g.ldr % 8 == 0));
   const long tiles256 = ((g.M + 255L) / 256) * ((g.N + 127L) / 128);
   if (tiles256 >= 512) {
-    if (vec) hipLaunchKernelGGL((mx_tile_kernel<256, true>), dim3((unsigned)tiles256), dim3(256), MXST * mx_stage<256>(), st, g);
-    else hipLaunchKernelGGL((mx_tile_kernel<256, false>), dim3((unsigned)tiles256), dim3(256), MXST * mx_stage<256>(), st, g);
+    if (vec) hipLaunchKernelGGL((mx_tile_kernel<256, true>), dim3((unsigned)tiles256), dim3(256), mx_lds<256>(), st, g);
+    else hipLaunchKernelGGL((mx_tile_kernel<256, false>), dim3((unsigned)tiles256), dim3(256), mx_lds<256>(), st, g);
   } else {
-    if (vec) hipLaunchKernelGGL((mx_tile_kernel<128, true>), dim3((unsigned)tiles), dim3(256), MXST * mx_stage<128>(), st, g);
-    else hipLaunchKernelGGL((mx_tile_kernel<128, false>), dim3((unsigned)tiles), dim3(256), MXST * mx_stage<128>(), st, g);
+    if (vec) hipLaunchKernelGGL((mx_tile_kernel<128, true>), dim3((unsigned)tiles), dim3(256), mx_lds<128>(), st, g);
+    else hipLaunchKernelGGL((mx_tile_kernel<128, false>), dim3((unsigned)tiles), dim3(256), mx_lds<128>(), st, g);
   }
 }
 
