@@ -61,6 +61,28 @@ __device__ __forceinline__ void gn_store8(void* p, long at, float (&f)[8]) {
   }
 }
 
+// Eight values as they lie in memory, so that all loads of a row are under way before the first is used.
+template <bool F32> struct Raw8;
+template <> struct Raw8<false> {
+  uint4 v;
+  __device__ __forceinline__ void load(const void* p, long at, bool on) {
+    v = on ? *reinterpret_cast<const uint4*>(reinterpret_cast<const bf16_t*>(p) + at) : make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const { unpack8(v, f); }
+};
+template <> struct Raw8<true> {
+  floatx4 a, b;
+  __device__ __forceinline__ void load(const void* p, long at, bool on) {
+    const float* q = reinterpret_cast<const float*>(p) + at;
+    a = on ? *reinterpret_cast<const floatx4*>(q) : floatx4{0.f, 0.f, 0.f, 0.f};
+    b = on ? *reinterpret_cast<const floatx4*>(q + 4) : floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = a[e], f[4 + e] = b[e];
+  }
+};
+
 // Sum over the TPR lanes (a power of two, at most 64) of a row, or over the whole block (TPR = 256) through `red`.
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float* red) {
@@ -87,50 +109,52 @@ __global__ __launch_bounds__(256) void gated_norm_fwd_kernel(GnArgs g) {
   for (int rb = r0; rb < r1; rb += RPB) {  // the same trip count for the whole block (row_sum's barriers)
     const bool ok = rb + sub < r1;
     const long row = (long)group * g.rows + rb + sub;
-    float u[NC][8], f[NC][8];
-    float ss = 0.f;
+    Raw8<false> wh[NC];
+    Raw8<XF32> wx[NC];
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int c = lane + TPR * i;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) u[i][e] = f[i][e] = 0.f;
-      if (ok && c < nch) {
-        gn_load8<false>(g.h, row * g.ldh + c * 8, u[i]);
-        gn_load8<XF32>(g.x, row * g.ldx + c * 8, f[i]);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ss += u[i][e] * u[i][e];
+      wh[i].load(g.h, row * g.ldh + c * 8, ok && c < nch);
+      wx[i].load(g.x, row * g.ldx + c * 8, ok && c < nch);
     }
-    float r = g.s;
+    float ss = 0.f, r = g.s;
     if (g.w_post) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        float u[8];
+        wh[i].get(u);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss += u[e] * u[e];
+      }
       const float rh = rsqrtf(row_sum<TPR>(ss, red) * inv + g.eps);
       if (lane == 0 && ok && g.rstd_post) g.rstd_post[row] = rh;
       r *= rh;
     }
+    float f[NC][8];
     ss = 0.f;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int c = lane + TPR * i;
-      if (c < nch) {
-        float t[8];
+      const int c = lane + TPR * i, cv = min(c, nch - 1);  // past the row: its last chunk's vectors, times zeros
+      float u[8], t[8];
+      wh[i].get(u);
+      wx[i].get(f[i]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) u[i][e] *= r;
-        if (g.w_post) {
-          gn_load8<false>(g.w_post, c * 8, t);
+      for (int e = 0; e < 8; ++e) u[e] *= r;
+      if (g.w_post) {
+        gn_load8<false>(g.w_post, cv * 8, t);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) u[i][e] *= t[e];
-        }
-        if (g.gate) {
-          gn_load8<false>(g.gate, group * g.ldg + c * 8, t);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) u[i][e] *= t[e];
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[i][e] += u[i][e];
-        if (ok) gn_store8<XF32>(g.xo, row * g.ldxo + c * 8, f[i]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss += f[i][e] * f[i][e];
+        for (int e = 0; e < 8; ++e) u[e] *= t[e];
       }
+      if (g.gate) {
+        gn_load8<false>(g.gate, group * g.ldg + cv * 8, t);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[e] *= t[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[i][e] += u[e];
+      if (ok && c < nch) gn_store8<XF32>(g.xo, row * g.ldxo + c * 8, f[i]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss += f[i][e] * f[i][e];
     }
     if (!g.w_pre) continue;
     const float rx = rsqrtf(row_sum<TPR>(ss, red) * inv + g.eps);
@@ -138,7 +162,7 @@ __global__ __launch_bounds__(256) void gated_norm_fwd_kernel(GnArgs g) {
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int c = lane + TPR * i;
-      if (c < nch) {
+      if (ok && c < nch) {
         float t[8];
         gn_load8<false>(g.w_pre, c * 8, t);
 #pragma unroll
@@ -150,17 +174,19 @@ __global__ __launch_bounds__(256) void gated_norm_fwd_kernel(GnArgs g) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) f[i][e] = f[i][e] * (1.f + t[e]) + b[e];
         }
-        if (ok) gn_store8<false>(g.y, row * g.ldy + c * 8, f[i]);
+        gn_store8<false>(g.y, row * g.ldy + c * 8, f[i]);
       }
     }
   }
 }
 
+constexpr int gn_bwd_occ(int nc) { return nc == 1 ? 4 : nc == 2 ? 3 : nc == 3 ? 2 : 1; }  // blocks per CU
+
 // The rows of a block belong to one group; each lane keeps the sums S, P, Q of its columns and the block leaves one partial
 // row of each in g.part (no atomics: the same bits every time).
 template <int TPR, int NC, bool XF32>
-__global__ __launch_bounds__(256) void gated_norm_bwd_kernel(GnArgs g) {
-  extern __shared__ __attribute__((aligned(16))) float cols[];  // [D], for the block's column sums
+__global__ __launch_bounds__(256, gn_bwd_occ(NC)) void gated_norm_bwd_kernel(GnArgs g) {
+  extern __shared__ __attribute__((aligned(16))) float cols[];  // [4][D], for the block's column sums
   __shared__ float red[4];
   constexpr int RPB = 256 / TPR;
   const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
@@ -176,78 +202,83 @@ __global__ __launch_bounds__(256) void gated_norm_bwd_kernel(GnArgs g) {
   for (int rb = r0; rb < r1; rb += RPB) {
     const bool ok = rb + sub < r1;
     const long row = (long)group * g.rows + rb + sub;
-    float dX[NC][8], n[NC][8], dn[NC][8];
+    Raw8<XF32> wx[NC], wd[NC];
+    Raw8<false> wy[NC], wh[NC];
     const float rx = ok && g.w_pre ? g.rstd_pre[row] : 0.f, rh = g.w_post ? (ok ? g.rstd_post[row] : 0.f) : 1.f;
-    float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int c = lane + TPR * i;
+      const bool on = ok && c < nch, pre = on && g.w_pre;
+      wx[i].load(g.x, row * g.ldx + c * 8, pre);
+      wy[i].load(g.dy, row * g.lddy + c * 8, pre);
+      wd[i].load(g.dxn, row * g.lddxn + c * 8, on && g.dxn);
+      wh[i].load(g.h, row * g.ldh + c * 8, on);
+    }
+    float dX[NC][8], dn[NC][8];
+    float dot = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) dX[i][e] = n[i][e] = dn[i][e] = 0.f;
-      if (ok && c < nch) {
-        if (g.dxn) gn_load8<XF32>(g.dxn, row * g.lddxn + c * 8, dX[i]);
-        if (g.w_pre) {
-          float t[8];
-          gn_load8<XF32>(g.x, row * g.ldx + c * 8, n[i]);
-          gn_load8<false>(g.dy, row * g.lddy + c * 8, dn[i]);
+    for (int i = 0; i < NC; ++i) {
+      const int c = min(lane + TPR * i, nch - 1);  // past the row: its last chunk's vectors, times zeros
+      wd[i].get(dX[i]);
+      if (g.w_pre) {
+        float n[8], t[8];
+        wx[i].get(n);
+        wy[i].get(dn[i]);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            n[i][e] *= rx;
-            S[i][e] += dn[i][e];
-            P[i][e] += dn[i][e] * n[i][e];
-          }
-          if (g.scale) {
-            gn_load8<false>(g.scale, group * g.lds + c * 8, t);
+        for (int e = 0; e < 8; ++e) {
+          n[e] *= rx;
+          S[i][e] += dn[i][e];
+          P[i][e] += dn[i][e] * n[e];
+        }
+        if (g.scale) {
+          gn_load8<false>(g.scale, group * g.lds + c * 8, t);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) dn[i][e] *= 1.f + t[e];
-          }
-          gn_load8<false>(g.w_pre, c * 8, t);
+          for (int e = 0; e < 8; ++e) dn[i][e] *= 1.f + t[e];
+        }
+        gn_load8<false>(g.w_pre, c * 8, t);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            dn[i][e] *= t[e];
-            dot += dn[i][e] * n[i][e];
-          }
+        for (int e = 0; e < 8; ++e) {
+          dn[i][e] *= t[e];
+          dot += dn[i][e] * n[e];
         }
       }
     }
     if (g.w_pre) {
       const float mean = row_sum<TPR>(dot, red) * inv;
 #pragma unroll
-      for (int i = 0; i < NC; ++i)
+      for (int i = 0; i < NC; ++i) {
+        float n[8];
+        wx[i].get(n);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) dX[i][e] += rx * (dn[i][e] - n[i][e] * mean);
+        for (int e = 0; e < 8; ++e) dX[i][e] += rx * (dn[i][e] - n[e] * rx * mean);
+      }
     }
-    // n, dn are free: n = v, dn = dv
     dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int c = lane + TPR * i;
+      const int c = lane + TPR * i, cv = min(c, nch - 1);
+      float v[8], t[8];
+      wh[i].get(v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) n[i][e] = dn[i][e] = 0.f;
-      if (ok && c < nch) {
-        float t[8];
-        gn_load8<false>(g.h, row * g.ldh + c * 8, n[i]);
+      for (int e = 0; e < 8; ++e) {
+        v[e] *= rh;
+        Q[i][e] += dX[i][e] * v[e];
+        dn[i][e] = dX[i][e] * g.s;  // from here on dn holds dv
+      }
+      if (g.gate) {
+        gn_load8<false>(g.gate, group * g.ldg + cv * 8, t);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dn[i][e] *= t[e];
+      }
+      if (g.w_post) {
+        gn_load8<false>(g.w_post, cv * 8, t);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          n[i][e] *= rh;
-          Q[i][e] += dX[i][e] * n[i][e];
-          dn[i][e] = dX[i][e] * g.s;
+          dn[i][e] *= t[e];
+          dot += dn[i][e] * v[e];
         }
-        if (g.gate) {
-          gn_load8<false>(g.gate, group * g.ldg + c * 8, t);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) dn[i][e] *= t[e];
-        }
-        if (g.w_post) {
-          gn_load8<false>(g.w_post, c * 8, t);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            dn[i][e] *= t[e];
-            dot += dn[i][e] * n[i][e];
-          }
-        }
-        if (g.xo) gn_store8<XF32>(g.xo, row * g.ldxo + c * 8, dX[i]);
       }
+      if (g.xo && ok && c < nch) gn_store8<XF32>(g.xo, row * g.ldxo + c * 8, dX[i]);
     }
     const float mean = g.w_post ? row_sum<TPR>(dot, red) * inv : 0.f;
 #pragma unroll
@@ -255,124 +286,139 @@ __global__ __launch_bounds__(256) void gated_norm_bwd_kernel(GnArgs g) {
       const int c = lane + TPR * i;
       if (ok && c < nch) {
         if (g.w_post) {
+          float v[8];
+          wh[i].get(v);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) dn[i][e] = rh * (dn[i][e] - n[i][e] * mean);
+          for (int e = 0; e < 8; ++e) dn[i][e] = rh * (dn[i][e] - v[e] * rh * mean);
         }
         gn_store8<false>(g.y, row * g.ldy + c * 8, dn[i]);
       }
     }
   }
   if (!g.part) return;
-  // column sums: the lanes of a wave that hold the same columns, then the waves in order through LDS
+  // column sums: the lanes of a wave that hold the same columns, then the four waves in order through LDS (cols [4][8 nch],
+  // value e of chunk c at e * nch + c: neighbouring lanes at neighbouring addresses)
   float* out = g.part + (long)blockIdx.x * 3 * g.D;
+  constexpr int WPR = TPR > 64 ? TPR / 64 : 1;  // waves per row: with more than one, every column has one lane
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
     float(&A)[NC][8] = k == 0 ? S : k == 1 ? P : Q;
-#pragma unroll
-    for (int i = 0; i < NC; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-#pragma unroll
-        for (int o = TPR; o < 64; o <<= 1) A[i][e] += __shfl_xor(A[i][e], o, 64);
-    if (TPR == 256) {  // every column has one lane
+    if (WPR > 1) {
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
         const int c = lane + TPR * i;
-        if (c < nch)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) out[k * g.D + c * 8 + e] = A[i][e];
+        if (c < nch) {
+          *reinterpret_cast<floatx4*>(out + k * g.D + c * 8) = floatx4{A[i][0], A[i][1], A[i][2], A[i][3]};
+          *reinterpret_cast<floatx4*>(out + k * g.D + c * 8 + 4) = floatx4{A[i][4], A[i][5], A[i][6], A[i][7]};
+        }
       }
       continue;
     }
-    for (int w = 0; w < 4; ++w) {
-      __syncthreads();
-      if ((int)threadIdx.x >> 6 == w && (threadIdx.x & 63) < TPR) {
+    __syncthreads();
+    float* mine = cols + (threadIdx.x >> 6) * g.D;
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-          const int c = lane + TPR * i;
-          if (c < nch)
+    for (int i = 0; i < NC; ++i) {
+      const int c = lane + TPR * i;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              if (w == 0) cols[c * 8 + e] = A[i][e];
-              else if (w < 3) cols[c * 8 + e] += A[i][e];
-              else out[k * g.D + c * 8 + e] = cols[c * 8 + e] + A[i][e];
-            }
-        }
+      for (int e = 0; e < 8; ++e) {
+#pragma unroll
+        for (int o = TPR; o < 64; o <<= 1) A[i][e] += __shfl_xor(A[i][e], o, 64);
+        if ((threadIdx.x & 63) < TPR && c < nch) mine[e * nch + c] = A[i][e];
       }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < nch; c += 256) {
+      float t[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float* q = cols + e * nch + c;
+        t[e] = (q[0] + q[g.D]) + (q[2 * g.D] + q[3 * g.D]);
+      }
+      *reinterpret_cast<floatx4*>(out + k * g.D + c * 8) = floatx4{t[0], t[1], t[2], t[3]};
+      *reinterpret_cast<floatx4*>(out + k * g.D + c * 8 + 4) = floatx4{t[4], t[5], t[6], t[7]};
     }
   }
 }
 
 struct GnSum {
   const float* part;  // [groups * bpg][3][D]
-  float* tot;         // [groups][3][D]
   const bf16_t* w_post; const bf16_t* w_pre;
   const bf16_t* gate; long ldg;
   const bf16_t* scale; long lds;
   float* dw_post; float* dw_pre;
   float* dgate; float* dscale; float* dshift;
-  int groups, bpg, D, gate_each, scale_each, shift_each;  // *_each: a gradient row per group
+  int groups, bpg, per, D, gate_each, scale_each, shift_each;  // *_each: a gradient row per group
   float s;
 };
 
-// tot[group][k][c] = sum over the group's blocks: 16 columns x 16 row slots per block, then a tree.
-__global__ __launch_bounds__(256) void gated_norm_sum_kernel(GnSum g) {
-  __shared__ float red[16][17];
-  const int cl = threadIdx.x & 15, rg = threadIdx.x >> 4;
-  const int c = blockIdx.x * 16 + cl, k = blockIdx.y, group = blockIdx.z;
-  float s = 0.f;
-  if (c < g.D)
-    for (int b = rg; b < g.bpg; b += 16) s += g.part[(((long)group * g.bpg + b) * 3 + k) * g.D + c];
-  red[rg][cl] = s;
-  __syncthreads();
+// The gradients of the vectors from the blocks' partial rows: block (x, k) takes 16 columns of sum k (0 S: dshift; 1 P: dscale,
+// dw_pre; 2 Q: dgate, dw_post), its 256 slots of 4 threads x 4 columns over (group, partial row). `per` slots (a power of two)
+// share a group, 256 / per groups go at once; the slots of a group meet in a tree, the groups one after the other: a fixed
+// order throughout.
+__global__ __launch_bounds__(1024) void gated_norm_vec_kernel(GnSum g) {
+  __shared__ floatx4 red[256][4];
+  const int k = blockIdx.y, cl = threadIdx.x & 3, slot = threadIdx.x >> 2;
+  float* each = k == 0 ? (g.shift_each ? g.dshift : nullptr) : k == 1 ? (g.scale_each ? g.dscale : nullptr)
+                                                                       : (g.gate_each ? g.dgate : nullptr);
+  float* sum = k == 0 ? (g.shift_each ? nullptr : g.dshift) : k == 1 ? (g.scale_each ? nullptr : g.dscale)
+                                                                      : (g.gate_each ? nullptr : g.dgate);
+  float* w = k == 0 ? nullptr : k == 1 ? g.dw_pre : g.dw_post;
+  if (!each && !sum && !w) return;
+  const int c = blockIdx.x * 16 + cl * 4;
+  const bool on = c < g.D;  // D % 8 == 0: all four columns or none
+  const int per = g.per, at_once = 256 / per, rank = slot & (per - 1);
+  // d(vector of each group) = mul * sum; d(norm weight) = sum over groups of fac * sum, fac = 1 + scale or s * gate
+  float mul[4] = {1.f, 1.f, 1.f, 1.f};
+  const bf16_t* wv = k == 1 ? g.w_pre : k == 2 ? g.w_post : nullptr;
 #pragma unroll
-  for (int st = 8; st >= 1; st >>= 1) {
-    if (rg < st) red[rg][cl] += red[rg + st][cl];
-    __syncthreads();
+  for (int e = 0; e < 4; ++e) {
+    if (on && wv) mul[e] = bf2f(wv[c + e]);
+    if (k == 2) mul[e] *= g.s;
   }
-  if (rg == 0 && c < g.D) g.tot[((long)group * 3 + k) * g.D + c] = red[0][cl];
-}
-
-// The gradients of the vectors from the groups' sums: 16 columns x 16 group slots per block, then a tree over the slots for
-// what all groups share.
-__global__ __launch_bounds__(256) void gated_norm_vec_kernel(GnSum g) {
-  __shared__ float red[5][16][17];
-  const int cl = threadIdx.x & 15, rg = threadIdx.x >> 4;
-  const int c = blockIdx.x * 16 + cl;
-  float a[5] = {0.f, 0.f, 0.f, 0.f, 0.f};  // dw_post, dw_pre, dgate, dscale, dshift
-  if (c < g.D) {
-    const float wp = g.w_post ? bf2f(g.w_post[c]) : 1.f, wn = g.w_pre ? bf2f(g.w_pre[c]) : 1.f;
-    for (int i = rg; i < g.groups; i += 16) {
-      const float* t = g.tot + (long)i * 3 * g.D + c;
-      const float S = t[0], P = t[g.D], Q = t[2 * g.D];
-      const float sc = g.scale ? bf2f(g.scale[i * g.lds + c]) : 0.f, gt = g.gate ? bf2f(g.gate[i * g.ldg + c]) : 1.f;
-      const float dg = g.s * wp * Q, ds = wn * P;
-      if (g.dgate && g.gate_each) g.dgate[(long)i * g.D + c] = dg;
-      if (g.dscale && g.scale_each) g.dscale[(long)i * g.D + c] = ds;
-      if (g.dshift && g.shift_each) g.dshift[(long)i * g.D + c] = S;
-      a[0] += g.s * gt * Q;
-      a[1] += (1.f + sc) * P;
-      a[2] += dg;
-      a[3] += ds;
-      a[4] += S;
+  const bf16_t* fv = k == 1 ? g.scale : k == 2 ? g.gate : nullptr;
+  const long fld = k == 1 ? g.lds : g.ldg;
+  float a_sum[4] = {0.f, 0.f, 0.f, 0.f}, a_w[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int g0 = 0; g0 < g.groups; g0 += at_once) {
+    const int i = g0 + slot / per;
+    floatx4 s = {0.f, 0.f, 0.f, 0.f};
+    if (on && i < g.groups) {
+      const float* p = g.part + ((long)i * g.bpg * 3 + k) * g.D + c;
+#pragma unroll 4
+      for (int b = rank; b < g.bpg; b += per) s += *reinterpret_cast<const floatx4*>(p + (long)b * 3 * g.D);
     }
-  }
+    red[slot][cl] = s;
+    __syncthreads();
+    for (int st = per >> 1; st >= 1; st >>= 1) {
+      if (rank < st) red[slot][cl] += red[slot + st][cl];
+      __syncthreads();
+    }
+    if (rank == 0 && on && i < g.groups) {
+      s = red[slot][cl];
 #pragma unroll
-  for (int k = 0; k < 5; ++k) red[k][rg][cl] = a[k];
-  __syncthreads();
-#pragma unroll
-  for (int st = 8; st >= 1; st >>= 1) {
-    if (rg < st)
-#pragma unroll
-      for (int k = 0; k < 5; ++k) red[k][rg][cl] += red[k][rg + st][cl];
+      for (int e = 0; e < 4; ++e) {
+        const float f = fv ? bf2f(fv[i * fld + c + e]) : k == 1 ? 0.f : 1.f;
+        const float d = mul[e] * s[e];
+        if (each) each[(long)i * g.D + c + e] = d;
+        a_sum[e] += d;
+        a_w[e] += (k == 1 ? 1.f + f : g.s * f) * s[e];
+      }
+    }
     __syncthreads();
   }
-  if (rg != 0 || c >= g.D) return;
-  if (g.dw_post) g.dw_post[c] = red[0][0][cl];
-  if (g.dw_pre) g.dw_pre[c] = red[1][0][cl];
-  if (g.dgate && !g.gate_each) g.dgate[c] = red[2][0][cl];
-  if (g.dscale && !g.scale_each) g.dscale[c] = red[3][0][cl];
-  if (g.dshift && !g.shift_each) g.dshift[c] = red[4][0][cl];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    float* out = t == 0 ? sum : w;
+    if (!out) continue;  // the same for the whole block
+    if (rank == 0) red[slot / per][cl] = t == 0 ? floatx4{a_sum[0], a_sum[1], a_sum[2], a_sum[3]}
+                                                : floatx4{a_w[0], a_w[1], a_w[2], a_w[3]};
+    __syncthreads();
+    if (slot == 0 && on) {
+      floatx4 v = {0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < at_once; ++i) v += red[i][cl];
+      *reinterpret_cast<floatx4*>(out + c) = v;
+    }
+    __syncthreads();
+  }
 }
 
 constexpr int kGnMaxD = 10240;
@@ -383,37 +429,71 @@ int gn_tpr(int D) {
   return nch <= 80 ? 16 : nch <= 160 ? 32 : nch <= 320 ? 64 : 256;
 }
 
+// The backward keeps three sums for each of a lane's columns, so at most 3 chunks per lane below 1536 columns (5 took 256
+// registers and one wave per SIMD).
+int gn_bwd_tpr(int D) { return D <= 384 ? 16 : D <= 1536 ? 64 : 256; }
+// Rows per block of the backward: whole passes of the block's rows, as many blocks as fit on the 256 CUs at once where there
+// are enough rows.
+int gn_rows_per_block(int groups, int rows, int D) {
+  const int tpr = gn_bwd_tpr(D), nc = (D / 8 + tpr - 1) / tpr;
+  const long rpb = 256 / tpr, at_once = 256L * gn_bwd_occ(nc) * rpb;
+  const long passes = ((long)groups * rows + at_once - 1) / at_once;
+  return (int)(rpb * (passes < 1 ? 1 : passes));
+}
 int gn_blocks_per_group(int groups, int rows, int D) {
-  const int rpb = 256 / gn_tpr(D);
-  const long want = ((long)rows + 4 * rpb - 1) / (4 * rpb), most = groups >= 1024 ? 1 : 1024 / groups;
-  return (int)(want < most ? (want < 1 ? 1 : want) : most);
+  const int rpb = gn_rows_per_block(groups, rows, D);
+  return (rows + rpb - 1) / rpb;
 }
 
 template <int TPR, int NC>
-void gn_launch(const GnArgs& g, int blocks, bool bwd, bool xf32, hipStream_t s) {
-  const size_t lds = TPR == 256 ? 0 : (size_t)g.D * sizeof(float);
-  if (bwd && xf32) hipLaunchKernelGGL((gated_norm_bwd_kernel<TPR, NC, true>), dim3(blocks), dim3(256), lds, s, g);
-  else if (bwd) hipLaunchKernelGGL((gated_norm_bwd_kernel<TPR, NC, false>), dim3(blocks), dim3(256), lds, s, g);
-  else if (xf32) hipLaunchKernelGGL((gated_norm_fwd_kernel<TPR, NC, true>), dim3(blocks), dim3(256), 0, s, g);
+void gn_fwd_launch(const GnArgs& g, int blocks, bool xf32, hipStream_t s) {
+  if (xf32) hipLaunchKernelGGL((gated_norm_fwd_kernel<TPR, NC, true>), dim3(blocks), dim3(256), 0, s, g);
   else hipLaunchKernelGGL((gated_norm_fwd_kernel<TPR, NC, false>), dim3(blocks), dim3(256), 0, s, g);
+}
+template <int TPR, int NC>
+void gn_bwd_launch(const GnArgs& g, int blocks, bool xf32, hipStream_t s) {
+  const size_t lds = TPR > 64 ? 0 : (size_t)g.D * 4 * sizeof(float);
+  if (xf32) hipLaunchKernelGGL((gated_norm_bwd_kernel<TPR, NC, true>), dim3(blocks), dim3(256), lds, s, g);
+  else hipLaunchKernelGGL((gated_norm_bwd_kernel<TPR, NC, false>), dim3(blocks), dim3(256), lds, s, g);
 }
 
 template <int TPR>
-void gn_chunks(const GnArgs& g, int blocks, bool bwd, bool xf32, hipStream_t s) {
-  const int nc = (g.D / 8 + TPR - 1) / TPR;
-  if (nc <= 1) gn_launch<TPR, 1>(g, blocks, bwd, xf32, s);
-  else if (nc == 2) gn_launch<TPR, 2>(g, blocks, bwd, xf32, s);
-  else if (nc == 3) gn_launch<TPR, 3>(g, blocks, bwd, xf32, s);
-  else if (nc == 4) gn_launch<TPR, 4>(g, blocks, bwd, xf32, s);
-  else gn_launch<TPR, 5>(g, blocks, bwd, xf32, s);
+void gn_fwd(const GnArgs& g, int blocks, bool xf32, hipStream_t s) {
+  switch ((g.D / 8 + TPR - 1) / TPR) {
+    case 1: gn_fwd_launch<TPR, 1>(g, blocks, xf32, s); break;
+    case 2: gn_fwd_launch<TPR, 2>(g, blocks, xf32, s); break;
+    case 3: gn_fwd_launch<TPR, 3>(g, blocks, xf32, s); break;
+    case 4: gn_fwd_launch<TPR, 4>(g, blocks, xf32, s); break;
+    default: gn_fwd_launch<TPR, 5>(g, blocks, xf32, s);
+  }
+}
+template <int TPR>
+void gn_bwd(const GnArgs& g, int blocks, bool xf32, hipStream_t s) {
+  switch ((g.D / 8 + TPR - 1) / TPR) {
+    case 1: gn_bwd_launch<TPR, 1>(g, blocks, xf32, s); break;
+    case 2: gn_bwd_launch<TPR, 2>(g, blocks, xf32, s); break;
+    case 3: gn_bwd_launch<TPR, 3>(g, blocks, xf32, s); break;
+    default:
+      if constexpr (TPR == 256) {
+        if (g.D <= 8192) gn_bwd_launch<TPR, 4>(g, blocks, xf32, s);
+        else gn_bwd_launch<TPR, 5>(g, blocks, xf32, s);
+      }
+  }
 }
 
-void gn_dispatch(const GnArgs& g, int blocks, bool bwd, bool xf32, hipStream_t s) {
+void gn_fwd_dispatch(const GnArgs& g, int blocks, bool xf32, hipStream_t s) {
   switch (gn_tpr(g.D)) {
-    case 16: gn_chunks<16>(g, blocks, bwd, xf32, s); break;
-    case 32: gn_chunks<32>(g, blocks, bwd, xf32, s); break;
-    case 64: gn_chunks<64>(g, blocks, bwd, xf32, s); break;
-    default: gn_chunks<256>(g, blocks, bwd, xf32, s);
+    case 16: gn_fwd<16>(g, blocks, xf32, s); break;
+    case 32: gn_fwd<32>(g, blocks, xf32, s); break;
+    case 64: gn_fwd<64>(g, blocks, xf32, s); break;
+    default: gn_fwd<256>(g, blocks, xf32, s);
+  }
+}
+void gn_bwd_dispatch(const GnArgs& g, int blocks, bool xf32, hipStream_t s) {
+  switch (gn_bwd_tpr(g.D)) {
+    case 16: gn_bwd<16>(g, blocks, xf32, s); break;
+    case 64: gn_bwd<64>(g, blocks, xf32, s); break;
+    default: gn_bwd<256>(g, blocks, xf32, s);
   }
 }
 
@@ -428,7 +508,7 @@ bool vec_ok(const void* p, long ld, int D) { return !p || (al16(p) && (ld == 0 |
 
 extern "C" long vpt_gated_norm_bwd_workspace(int groups, int rows, int D) {
   if (groups <= 0 || rows <= 0 || D <= 0 || D % 8 || D > kGnMaxD) return 0;
-  return ((long)groups * gn_blocks_per_group(groups, rows, D) + groups) * 3 * D * (long)sizeof(float);
+  return (long)groups * gn_blocks_per_group(groups, rows, D) * 3 * D * (long)sizeof(float);
 }
 
 #define VPT_GN_SHAPE(name)                                                                                             \
@@ -467,7 +547,7 @@ extern "C" int vpt_gated_norm_fwd(const void* h, long ldh, const void* x, int x_
   g.rpb = 256 / gn_tpr(D);
   g.bpg = (rows + g.rpb - 1) / g.rpb;
   g.s = resid_scale; g.eps = eps;
-  gn_dispatch(g, groups * g.bpg, false, x_f32 != 0, (hipStream_t)stream);
+  gn_fwd_dispatch(g, groups * g.bpg, x_f32 != 0, (hipStream_t)stream);
   VPT_LAUNCH_CHECK();
   return VPT_OK;
 }
@@ -497,7 +577,7 @@ extern "C" int vpt_gated_norm_bwd(const void* dy, long lddy, const void* dx_new,
   z.groups = groups; z.D = D;
   z.gate_each = ldg != 0; z.scale_each = lds != 0; z.shift_each = ldsh != 0;
   z.s = resid_scale;
-  VPT_CHECK_ARG(groups <= 65535, "vpt_gated_norm_bwd: at most 65535 groups");
+  VPT_CHECK_ARG((long)groups * gn_blocks_per_group(groups, rows > 0 ? rows : 1, D) < (1L << 31), "vpt_gated_norm_bwd: too many groups");
   VPT_CHECK_ARG(M > 0 || !sums, "vpt_gated_norm_bwd: no rows to sum over");
   if (M == 0) return VPT_OK;
   VPT_CHECK_ARG(h && dh && (!w_post || rstd_post) && (!w_pre || (dy && x_new && rstd_pre && dx)) && (w_pre || dx_new),
@@ -519,18 +599,17 @@ extern "C" int vpt_gated_norm_bwd(const void* dy, long lddy, const void* dx_new,
   g.rstd_post = const_cast<float*>(rstd_post); g.rstd_pre = const_cast<float*>(rstd_pre);
   g.rows = rows; g.D = D; g.s = resid_scale;
   g.bpg = gn_blocks_per_group(groups, rows, D);
-  g.rpb = (rows + g.bpg - 1) / g.bpg;
+  g.rpb = gn_rows_per_block(groups, rows, D);
   g.part = sums ? (float*)workspace : nullptr;
   const int blocks = groups * g.bpg;
-  gn_dispatch(g, blocks, true, x_f32 != 0, st);
+  gn_bwd_dispatch(g, blocks, x_f32 != 0, st);
   VPT_LAUNCH_CHECK();
   if (!sums) return VPT_OK;
   z.bpg = g.bpg;
   z.part = g.part;
-  z.tot = g.part + (long)blocks * 3 * D;
-  hipLaunchKernelGGL(gated_norm_sum_kernel, dim3((D + 15) / 16, 3, groups), dim3(256), 0, st, z);
-  VPT_LAUNCH_CHECK();
-  hipLaunchKernelGGL(gated_norm_vec_kernel, dim3((D + 15) / 16), dim3(256), 0, st, z);
+  z.per = 1;
+  while (z.per < 256 && z.per * 2 * groups <= 256) z.per *= 2;
+  hipLaunchKernelGGL(gated_norm_vec_kernel, dim3((D + 15) / 16, 3), dim3(1024), 0, st, z);
   VPT_LAUNCH_CHECK();
   return VPT_OK;
 }

@@ -22,6 +22,9 @@ struct Piece {  // include/vpt_hip.h VptGradPiece
   int n, dtype;
 };
 
+template <int T> constexpr int gc_size() { return T == GC_F32 ? 4 : 2; }
+template <int T> constexpr int gc_vec() { return 16 / gc_size<T>(); }  // values of 16 bytes
+
 template <int T>
 __device__ __forceinline__ float gc_get(const void* p, int i) {
   return T == GC_F32    ? reinterpret_cast<const float*>(p)[i]
@@ -34,6 +37,33 @@ __device__ __forceinline__ void gc_put(void* p, int i, float v) {
   else if (T == GC_BF16) reinterpret_cast<bf16_t*>(p)[i] = f2bf(v);
   else reinterpret_cast<unsigned short*>(p)[i] = f2h(v);
 }
+template <int T>
+__device__ __forceinline__ void gc_unpack(uint4 v, float (&f)[gc_vec<T>()]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (T == GC_F32) f[e] = __uint_as_float(w[e]);
+    else if constexpr (T == GC_BF16) f[2 * e] = __uint_as_float(w[e] << 16), f[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+    else f[2 * e] = h2f(w[e] & 0xffff), f[2 * e + 1] = h2f(w[e] >> 16);
+  }
+}
+template <int T>
+__device__ __forceinline__ uint4 gc_pack(const float (&f)[gc_vec<T>()]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (T == GC_F32) w[e] = __float_as_uint(f[e]);
+    else if constexpr (T == GC_BF16) w[e] = pack_bf16x2(f[2 * e], f[2 * e + 1]);
+    else w[e] = f2h(f[2 * e]) | (uint32_t)f2h(f[2 * e + 1]) << 16;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// Values before the first 16-byte boundary of p (at most n).
+template <int T>
+__device__ __forceinline__ int gc_head(const void* p, int n) {
+  const int k = (int)((-(uintptr_t)p & 15) / gc_size<T>());
+  return k < n ? k : n;
+}
 
 __device__ __forceinline__ double block_sum(double v) {  // 256 threads; the result in every thread
   __shared__ double red[4];
@@ -45,12 +75,32 @@ __device__ __forceinline__ double block_sum(double v) {  // 256 threads; the res
   return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
+// 16-byte loads, four per thread in flight; the values before the first boundary and behind the last one apart.
 template <int T>
 __device__ __forceinline__ double piece_sumsq(const Piece& p) {
+  constexpr int V = gc_vec<T>(), U = 4;
+  const int head = gc_head<T>(p.g, p.n), nv = (p.n - head) / V, tail = head + nv * V;
   double s = 0.;
-  for (int i = threadIdx.x; i < p.n; i += 256) {
-    const double v = gc_get<T>(p.g, i);
+  if ((int)threadIdx.x < head) {
+    const double v = gc_get<T>(p.g, threadIdx.x);
     s += v * v;
+  }
+  if (tail + (int)threadIdx.x < p.n) {
+    const double v = gc_get<T>(p.g, tail + threadIdx.x);
+    s += v * v;
+  }
+  const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p.g) + head * gc_size<T>());
+  for (int i = threadIdx.x; i < nv; i += 256 * U) {
+    uint4 w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) w[u] = i + 256 * u < nv ? q[i + 256 * u] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float f[V];
+      gc_unpack<T>(w[u], f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) s = fma((double)f[e], (double)f[e], s);
+    }
   }
   return s;
 }
@@ -72,12 +122,33 @@ __device__ __forceinline__ double parts_norm(const double* part, int n) {
   return sqrt(block_sum(s));
 }
 
+__device__ __forceinline__ float gc_clip(float v, float coef, float limit) {
+  v *= coef;
+  return limit > 0.f ? (v < -limit ? -limit : v > limit ? limit : v) : v;  // a NaN stays one
+}
 template <int T>
 __device__ __forceinline__ void piece_clip(const Piece& p, float coef, float limit) {
-  for (int i = threadIdx.x; i < p.n; i += 256) {
-    float v = gc_get<T>(p.g, i) * coef;
-    if (limit > 0.f) v = v < -limit ? -limit : v > limit ? limit : v;  // a NaN stays one
-    gc_put<T>(p.out, i, v);
+  constexpr int V = gc_vec<T>(), U = 4;
+  int head = gc_head<T>(p.g, p.n), nv = (p.n - head) / V;
+  if (((uintptr_t)p.g ^ (uintptr_t)p.out) & 15) head = p.n, nv = 0;  // no 16-byte pieces in common: value by value
+  const int tail = head + nv * V;
+  for (int i = threadIdx.x; i < head; i += 256) gc_put<T>(p.out, i, gc_clip(gc_get<T>(p.g, i), coef, limit));
+  for (int i = tail + threadIdx.x; i < p.n; i += 256) gc_put<T>(p.out, i, gc_clip(gc_get<T>(p.g, i), coef, limit));
+  const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p.g) + (long)head * gc_size<T>());
+  uint4* o = reinterpret_cast<uint4*>(reinterpret_cast<char*>(p.out) + (long)head * gc_size<T>());
+  for (int i = threadIdx.x; i < nv; i += 256 * U) {
+    uint4 w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) w[u] = i + 256 * u < nv ? q[i + 256 * u] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float f[V];
+      gc_unpack<T>(w[u], f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[e] = gc_clip(f[e], coef, limit);
+      w[u] = gc_pack<T>(f);
+      if (i + 256 * u < nv) o[i + 256 * u] = w[u];
+    }
   }
 }
 
@@ -94,7 +165,7 @@ __global__ __launch_bounds__(256) void grad_list_clip_kernel(const Piece* __rest
     }
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
   }
-  for (int i = blockIdx.x; i < count; i += gridDim.x) {
+  for (int i = count - 1 - (int)blockIdx.x; i >= 0; i -= gridDim.x) {  // last read, first again: what the caches still hold
     const Piece p = pieces[i];
     if (coef == 1.f && limit <= 0.f && p.out == p.g) continue;  // in place and nothing changes
     if (p.dtype == GC_F32) piece_clip<GC_F32>(p, coef, limit);

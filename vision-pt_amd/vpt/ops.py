@@ -1566,7 +1566,6 @@ def gated_norm_bwd(dy, dx_new, h, x_new, rstd_post, rstd_pre, *, w_post=None, w_
     M, D = h.shape
     _gn_params(fn, D, M, groups, w_post, w_pre, gate, scale, shift)
     _rows2d(h, fn, "h", _BF16, (M, D), 16)
-    _need(groups <= 65535, "gated_norm_bwd: at most 65535 groups")
     _need((dy is None) == (w_pre is None), "gated_norm_bwd: dy goes with w_pre")
     if w_pre is not None:
         _rows2d(x_new, fn, "x_new", _MX_OUT, (M, D), 16)
