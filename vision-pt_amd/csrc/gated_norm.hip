@@ -186,7 +186,7 @@ constexpr int gn_bwd_occ(int nc) { return nc == 1 ? 4 : nc == 2 ? 3 : nc == 3 ? 
 // row of each in g.part (no atomics: the same bits every time).
 template <int TPR, int NC, bool XF32>
 __global__ __launch_bounds__(256, gn_bwd_occ(NC)) void gated_norm_bwd_kernel(GnArgs g) {
-  extern __shared__ __attribute__((aligned(16))) float cols[];  // [4][D], for the block's column sums
+  extern __shared__ __attribute__((aligned(16))) float cols[];  // the rows' factors [2][D], then column sums [4][D]
   __shared__ float red[4];
   constexpr int RPB = 256 / TPR;
   const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
@@ -194,6 +194,37 @@ __global__ __launch_bounds__(256, gn_bwd_occ(NC)) void gated_norm_bwd_kernel(GnA
   const int nch = g.D >> 3;
   const float inv = 1.f / (float)g.D;
   const int r1 = min(g.rows, r0 + g.rpb);
+  // what the rows of the group share: (1 + scale) w_pre and s gate w_post, f32
+  float* cw = cols;
+  float* gw = cols + g.D;
+  for (int c = threadIdx.x; c < nch; c += 256) {
+    float a[8], b[8], t[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a[e] = 1.f, b[e] = g.s;
+    if (g.scale) {
+      gn_load8<false>(g.scale, group * g.lds + c * 8, t);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a[e] += t[e];
+    }
+    if (g.w_pre) {
+      gn_load8<false>(g.w_pre, c * 8, t);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a[e] *= t[e];
+    }
+    if (g.gate) {
+      gn_load8<false>(g.gate, group * g.ldg + c * 8, t);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) b[e] *= t[e];
+    }
+    if (g.w_post) {
+      gn_load8<false>(g.w_post, c * 8, t);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) b[e] *= t[e];
+    }
+    gn_store8<true>(cw, c * 8, a);
+    gn_store8<true>(gw, c * 8, b);
+  }
+  __syncthreads();
   float S[NC][8], P[NC][8], Q[NC][8];
 #pragma unroll
   for (int i = 0; i < NC; ++i)
@@ -218,11 +249,12 @@ __global__ __launch_bounds__(256, gn_bwd_occ(NC)) void gated_norm_bwd_kernel(GnA
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int c = min(lane + TPR * i, nch - 1);  // past the row: its last chunk's vectors, times zeros
+      const int c = min(lane + TPR * i, nch - 1);  // past the row: its last chunk's factors, times zeros
       wd[i].get(dX[i]);
       if (g.w_pre) {
         float n[8], t[8];
         wx[i].get(n);
+        gn_load8<true>(cw, c * 8, t);
         wy[i].get(dn[i]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -230,12 +262,6 @@ __global__ __launch_bounds__(256, gn_bwd_occ(NC)) void gated_norm_bwd_kernel(GnA
           S[i][e] += dn[i][e];
           P[i][e] += dn[i][e] * n[e];
         }
-        if (g.scale) {
-          gn_load8<false>(g.scale, group * g.lds + c * 8, t);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) dn[i][e] *= 1.f + t[e];
-        }
-        gn_load8<false>(g.w_pre, c * 8, t);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           dn[i][e] *= t[e];
@@ -259,24 +285,13 @@ __global__ __launch_bounds__(256, gn_bwd_occ(NC)) void gated_norm_bwd_kernel(GnA
       const int c = lane + TPR * i, cv = min(c, nch - 1);
       float v[8], t[8];
       wh[i].get(v);
+      gn_load8<true>(gw, cv * 8, t);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         v[e] *= rh;
         Q[i][e] += dX[i][e] * v[e];
-        dn[i][e] = dX[i][e] * g.s;  // from here on dn holds dv
-      }
-      if (g.gate) {
-        gn_load8<false>(g.gate, group * g.ldg + cv * 8, t);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) dn[i][e] *= t[e];
-      }
-      if (g.w_post) {
-        gn_load8<false>(g.w_post, cv * 8, t);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          dn[i][e] *= t[e];
-          dot += dn[i][e] * v[e];
-        }
+        dn[i][e] = dX[i][e] * t[e];  // from here on dn holds dv
+        dot += dn[i][e] * v[e];
       }
       if (g.xo && ok && c < nch) gn_store8<XF32>(g.xo, row * g.ldxo + c * 8, dX[i]);
     }
@@ -452,7 +467,7 @@ void gn_fwd_launch(const GnArgs& g, int blocks, bool xf32, hipStream_t s) {
 }
 template <int TPR, int NC>
 void gn_bwd_launch(const GnArgs& g, int blocks, bool xf32, hipStream_t s) {
-  const size_t lds = TPR > 64 ? 0 : (size_t)g.D * 4 * sizeof(float);
+  const size_t lds = (size_t)g.D * (TPR > 64 ? 2 : 4) * sizeof(float);
   if (xf32) hipLaunchKernelGGL((gated_norm_bwd_kernel<TPR, NC, true>), dim3(blocks), dim3(256), lds, s, g);
   else hipLaunchKernelGGL((gated_norm_bwd_kernel<TPR, NC, false>), dim3(blocks), dim3(256), lds, s, g);
 }
