@@ -128,8 +128,8 @@ def test_c_abi_refuses_clip(m):
     p = 4096
     assert lib.vpt_grad_list_norm(p, -1, p, None) == 1 and lib.vpt_grad_list_norm(None, 3, p, None) == 1
     assert lib.vpt_grad_list_norm(p, 3, None, None) == 1 and lib.vpt_grad_list_norm(p, 3, p + 4, None) == 1
-    ok = [p, 3, p, 3, 1.0, 0.0, p, None]
-    for i, v in [(0, None), (1, -1), (2, None), (2, p + 4), (3, 0), (3, 1 << 20), (4, -1.0), (5, -1.0), (4, float("nan"))]:
+    ok = [p, 3, 0, p, 3, 1.0, 0.0, p, None]
+    for i, v in [(0, None), (1, -1), (3, None), (3, p + 4), (4, 0), (4, 1 << 20), (5, -1.0), (6, -1.0), (5, float("nan"))]:
         a = list(ok)
         a[i] = v
         assert lib.vpt_grad_list_clip(*a) == 1, (i, v)

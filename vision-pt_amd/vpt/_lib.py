@@ -117,7 +117,7 @@ SIGNATURES: dict[str, list] = {
     "vpt_grad_list_piece": [],
     "vpt_grad_list_parts": [I],
     "vpt_grad_list_norm": [P, I, P, P],
-    "vpt_grad_list_clip": [P, I, P, I, F, F, P, P],
+    "vpt_grad_list_clip": [P, I, I, P, I, F, F, P, P],
     "vpt_mxfp4_quantize": [P, I, L, L, I, P, L, P, L, P],
     "vpt_mxfp4_dequantize": [P, L, P, L, L, I, P, L, I, P],
     "vpt_gemm_mxfp4": [P, L, P, L, P, L, P, L, P, L, I, I, I, P, P, L, I, P],

@@ -200,6 +200,7 @@ class GradClip:
             self._table, self._count = self._pieces()
             self._stream = ops._raw_stream(self.device.index)
         self._parts = ops.call("vpt_grad_list_parts", self._count)
+        self._in_place = int(all(o.data_ptr() == g.data_ptr() for g, o in zip(self.grads, self.out)))
 
     def _pieces(self):
         piece = ops.call("vpt_grad_list_piece")
@@ -225,12 +226,13 @@ class GradClip:
                 self._table.record_stream(torch.cuda.current_stream())
             table = None if self._table is None else self._table.data_ptr()
             if not want_norm:
-                ops.call("vpt_grad_list_clip", table, count, None, 0, 0.0, clip_value, None, st)
+                ops.call("vpt_grad_list_clip", table, count, self._in_place, None, 0, 0.0, clip_value, None, st)
                 return None
             ws = torch.empty(self._parts + 1, dtype=torch.float64, device=self.device)
             norm = ws[self._parts:].view(torch.float32)[0]
             ops.call("vpt_grad_list_norm", table, self._count, ws.data_ptr(), st)
-            ops.call("vpt_grad_list_clip", table, count, ws.data_ptr(), self._parts, max_norm, clip_value, norm.data_ptr(), st)
+            ops.call("vpt_grad_list_clip", table, count, self._in_place, ws.data_ptr(), self._parts, max_norm, clip_value,
+                     norm.data_ptr(), st)
             return norm
 
     @torch.no_grad()
