@@ -362,3 +362,13 @@ def test_repeatable(m):
     for M in (1, 30, 300):
         x, _, b, r, w, y = product(m, M, 520, 1000, seed=M)
         assert all(torch.equal(ops.linear_mxfp4(x, w, bias=b, resid=r), y) for _ in range(5))
+
+
+@pytest.mark.parametrize("M,N,K", [(M, N, K) for M, N in [(4100, 4104), (8193, 2049), (1200, 1032), (1100, 515)]
+                                   for K in (100, 256, 300, 512, 600, 768, 800, 1100)] +
+                         [(4000, 4000, K) for K in (2945, 3100, 3200, 3300, 3456)] + [(3900, 4001, 3100)])
+def test_linear_large(m, M, N, K):
+    """Grids of every tile kernel (256 x 256 from 24 steps along K on), one step to nine, edges in both directions."""
+    x, wt, b, r, w, y = product(m, M, N, K, seed=K, out_dtype=F32 if K == 300 else BF16)
+    close(y, x, wt, b, r)
+    assert torch.equal(m[0].linear_mxfp4(x, w, bias=b, resid=r, out_dtype=y.dtype), y)

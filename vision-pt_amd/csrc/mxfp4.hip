@@ -206,56 +206,91 @@ __device__ __forceinline__ void mx_issue_scales(const MxArgs& g, const MxOffs& o
   glds16(uniform_ptr(g.BS + (long)n0 * g.ldbs + at), o.bs, __builtin_amdgcn_readfirstlane(ls + TM * 16 + (wid & 1) * 1024));
 }
 
+// The scale bytes of block blk in the 4 steps whose 16 bytes lie at p: byte s of the result is step s's. `first` > 0: the steps
+// are the last 4 - first of the row, at the end of the 16 bytes.
+__device__ __forceinline__ uint32_t mx_scale4(const char* p, uint32_t sel_lo, uint32_t sel_hi, int first) {
+  const uint4 d = *reinterpret_cast<const uint4*>(p);
+  return (__builtin_amdgcn_perm(d.y, d.x, sel_lo) | __builtin_amdgcn_perm(d.w, d.z, sel_hi)) >> (8 * first);
+}
+
 template <int S>
 __device__ __forceinline__ floatx4 mx_mfma_at(uint4 a, uint4 b, floatx4 c, uint32_t sa, uint32_t sb) {  // scale byte S
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_frag(a), mx_frag(b), c, 4, 4, S, (int)sa, S, (int)sb);
 }
 
-// acc[i][j][e]: row 16 i + (lane & 15), column 32 (j >> 1) + 8 (lane >> 4) + 4 (j & 1) + e of the wave's tile. VEC: 16-byte
-// accesses (N % 8 == 0, 16-byte rows), else element by element.
-template <bool VEC, int MI>
-__device__ __forceinline__ void mx_epilogue(const MxArgs& g, const floatx4 (&acc)[MI][4], int lane, int row0, int col0,
-                                            const float (&bias)[2][8]) {
-  const int c0 = col0 + (lane >> 4) * 8;
+// acc[i][j][e]: row 16 i + (lane & 15), column 32 (j >> 1) + 8 (lane >> 4) + 4 (j & 1) + e of the wave's tile, which starts at
+// (row0, col0) of the block's at (m0, n0). VEC (N % 8 == 0, 16-byte rows): 16-byte buffer stores whose per-store part is one
+// scalar; rows past M lie behind the buffer's end, columns past N get an offset there, and the hardware drops them. Otherwise
+// element by element.
+template <bool VEC, int AUX, int MI, int NP>
+__device__ __forceinline__ void mx_epilogue(const MxArgs& g, const floatx4 (&acc)[MI][2 * NP], int lane, int m0, int n0, int row0,
+                                            int col0, const float (&bias)[NP][8]) {
+  const int lr = row0 + (lane & 15), lc = col0 + (lane >> 4) * 8;
+  if (VEC) {
+    const int es = g.f32out ? 4 : 2, rows_here = min(256, g.M - m0);
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+        (char*)g.C + ((long)m0 * g.ldc + n0) * es, (short)0, rows_here * (int)g.ldc * es, 0x00020000);
+    const bf16_t* rbase = g.resid ? g.resid + (long)m0 * g.ldr + n0 : nullptr;
+    const __amdgpu_buffer_rsrc_t rr = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)rbase, (short)0, g.resid ? rows_here * (int)g.ldr * 2 : 0, 0x00020000);
+    uint32_t vo[NP], vr[NP];
 #pragma unroll
-  for (int i = 0; i < MI; ++i) {
-    const int row = row0 + i * 16 + (lane & 15);
-    if (row >= g.M) continue;
+    for (int q = 0; q < NP; ++q) {
+      const bool in = n0 + lc + q * 32 < g.N;
+      vo[q] = in ? (uint32_t)((lr * (int)g.ldc + lc + q * 32) * es) : 0x80000000u;
+      vr[q] = in ? (uint32_t)((lr * (int)g.ldr + lc + q * 32) * 2) : 0x80000000u;
+    }
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int col = c0 + q * 32;
-      float o[8];
+    for (int i = 0; i < MI; ++i) {
+      u32x4 res[NP];
+      if (g.resid) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = acc[i][2 * q + (e >> 2)][e & 3] + bias[q][e];
-      if (VEC) {
-        if (col >= g.N) continue;
+        for (int q = 0; q < NP; ++q) res[q] = __builtin_amdgcn_raw_buffer_load_b128(rr, (int)vr[q], i * 32 * (int)g.ldr, 0);
+      }
+      const int so = i * 16 * (int)g.ldc * es;
+#pragma unroll
+      for (int q = 0; q < NP; ++q) {
+        float o[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = acc[i][2 * q + (e >> 2)][e & 3] + bias[q][e];
         if (g.resid) {
           float rv[8];
-          unpack8(*reinterpret_cast<const uint4*>(g.resid + (long)row * g.ldr + col), rv);
+          unpack8(make_uint4(res[q][0], res[q][1], res[q][2], res[q][3]), rv);
 #pragma unroll
           for (int e = 0; e < 8; ++e) o[e] += rv[e];
         }
         if (g.f32out) {
-          float* c = reinterpret_cast<float*>(g.C) + (long)row * g.ldc + col;
-          *reinterpret_cast<floatx4*>(c) = floatx4{o[0], o[1], o[2], o[3]};
-          *reinterpret_cast<floatx4*>(c + 4) = floatx4{o[4], o[5], o[6], o[7]};
+          store_b128_padded<AUX>(u32x4{__float_as_uint(o[0]), __float_as_uint(o[1]), __float_as_uint(o[2]), __float_as_uint(o[3])},
+                                 rs, (int)vo[q], so);
+          store_b128_padded<AUX>(u32x4{__float_as_uint(o[4]), __float_as_uint(o[5]), __float_as_uint(o[6]), __float_as_uint(o[7])},
+                                 rs, (int)vo[q], so + 16);
         } else {
-          *reinterpret_cast<uint4*>(reinterpret_cast<bf16_t*>(g.C) + (long)row * g.ldc + col) = pack8(o);
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (col + e >= g.N) break;
-          if (g.resid) o[e] += bf2f(g.resid[(long)row * g.ldr + col + e]);
-          if (g.f32out) reinterpret_cast<float*>(g.C)[(long)row * g.ldc + col + e] = o[e];
-          else reinterpret_cast<bf16_t*>(g.C)[(long)row * g.ldc + col + e] = f2bf(o[e]);
+          const uint4 w = pack8(o);
+          store_b128_padded<AUX>(u32x4{w.x, w.y, w.z, w.w}, rs, (int)vo[q], so);
         }
       }
     }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int row = m0 + lr + i * 16;
+    if (row >= g.M) continue;
+#pragma unroll
+    for (int q = 0; q < NP; ++q)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int col = n0 + lc + q * 32 + e;
+        if (col >= g.N) break;
+        float o = acc[i][2 * q + (e >> 2)][e & 3] + bias[q][e];
+        if (g.resid) o += bf2f(g.resid[(long)row * g.ldr + col]);
+        if (g.f32out) reinterpret_cast<float*>(g.C)[(long)row * g.ldc + col] = o;
+        else reinterpret_cast<bf16_t*>(g.C)[(long)row * g.ldc + col] = f2bf(o);
+      }
   }
 }
 
-template <int TM, bool VEC>
+template <int TM, bool VEC, int AUX>
 __global__ __launch_bounds__(256, 2) void mx_tile_kernel(MxArgs g) {
   constexpr int MI = TM / 32, STG = mx_stage<TM>(), PCS = TM / 64 + 2;
   static_assert(PCS == 6 || PCS == 4, "the counted waits below");
@@ -268,6 +303,8 @@ __global__ __launch_bounds__(256, 2) void mx_tile_kernel(MxArgs g) {
   const int m0 = tile / tiles_n * TM, n0 = tile % tiles_n * 128;
   const uint32_t smem0 = (uint32_t)(uintptr_t)(VPT_LDS char*)smem;
   const int nk = g.steps, r = lane & 15, blk = lane >> 4;
+  // v_perm selectors: byte blk of one dword into byte 0 (2), of the next into byte 1 (3), zeros elsewhere
+  const uint32_t sel_lo = 0x0c0c0400u + blk * 0x0101u, sel_hi = 0x04000c0cu + blk * 0x01010000u;
   MxOffs o;  // rows past the edge: the last one (its results are not stored)
 #pragma unroll
   for (int i = 0; i < TM / 64; ++i) o.a[i] = tile_voff<true, TM, 4>(g.lda >> 1, m0, g.M, RBK, wid, lane, i);
@@ -330,22 +367,12 @@ __global__ __launch_bounds__(256, 2) void mx_tile_kernel(MxArgs g) {
     if (kt + 2 < nk) mx_issue<TM>(g, o, m0, n0, kt + 2, smem0, wid);
     const char* st = smem + (kt % MXST) * STG;
     if (S == 0 && nk >= 4) {
-      const char* sc = smem + MXST * STG + blk;
+      const char* sc = smem + MXST * STG;
       const int rem = nk - kt, first = rem < 4 ? 4 - rem : 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint8_t* p = reinterpret_cast<const uint8_t*>(sc + TM * 16 + (wn * 64 + j * 16 + r) * 16);
-        sb[j] = 0;
+      for (int j = 0; j < 4; ++j) sb[j] = mx_scale4(sc + TM * 16 + (wn * 64 + j * 16 + r) * 16, sel_lo, sel_hi, first);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sb[j] |= (uint32_t)p[min(first + e, 3) * 4] << (8 * e);
-      }
-#pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        const uint8_t* p = reinterpret_cast<const uint8_t*>(sc + (wm * (TM / 2) + i * 16 + r) * 16);
-        sa[i] = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sa[i] |= (uint32_t)p[min(first + e, 3) * 4] << (8 * e);
-      }
+      for (int i = 0; i < MI; ++i) sa[i] = mx_scale4(sc + (wm * (TM / 2) + i * 16 + r) * 16, sel_lo, sel_hi, first);
     }
     uint4 af[MI], bf[4];
 #pragma unroll
@@ -380,7 +407,138 @@ __global__ __launch_bounds__(256, 2) void mx_tile_kernel(MxArgs g) {
     if (kt + 2 < nk) step(kt + 2, std::integral_constant<int, 2>{});
     if (kt + 3 < nk) step(kt + 3, std::integral_constant<int, 3>{});
   }
-  mx_epilogue<VEC, MI>(g, acc, lane, m0 + wm * (TM / 2), n0 + wn * 64, bias);
+  mx_epilogue<VEC, AUX, MI, 2>(g, acc, lane, m0, n0, wm * (TM / 2), wn * 64, bias);
+}
+
+// ---- large products: 256 x 256 tiles, 8 waves (2 x 4) of 128 x 64, one block per CU -----------------------------------
+// The same wave tile as the 256 x 128 form with two thirds of its LDS-DMA per product, four stages (three steps ahead), and the
+// phases of the bf16 256x256 ring (gemm.hip): waves 4-7 run one barrier behind waves 0-3, so that on every SIMD one wave
+// multiplies while the other reads its fragments.
+//   L_t: DMA of step t + 3 into the stage of step t - 1; fragments of step t into registers; this wave's pieces of step
+//        t + 1 have landed; barrier      C_t: 32 MFMAs; barrier
+// A stage is refilled in L_t, after both groups' L_t-1 closed with lgkmcnt(0) and a barrier; a step's pieces of all waves have
+// landed one barrier before the first group reads them. The scales' buffer (one, 16 bytes per row) is read in L_4c and
+// refilled from L_4c+1 on; its piece has landed where step 4c + 4's are waited for.
+constexpr int MXR_ST = 4, MXR_STG = 512 * 64;
+constexpr int mx_ring_lds() { return MXR_ST * MXR_STG + 512 * 16; }  // 136 KB
+
+__device__ __forceinline__ void mxr_issue(const MxArgs& g, const uint32_t (&va)[2], const uint32_t (&vb)[2], int m0, int n0, int t,
+                                          uint32_t smem0, int wid) {
+  const uint32_t la = __builtin_amdgcn_readfirstlane(smem0 + (uint32_t)(t % MXR_ST) * MXR_STG + wid * 2048);
+  glds_step(uniform_ptr(g.A + (long)m0 * g.lda + t * 64), uniform_ptr(g.B + (long)n0 * g.ldb + t * 64), va[0], va[1], vb[0],
+            vb[1], la, la + 1024, la + 16384, la + 16384 + 1024);
+}
+
+template <bool VEC, int AUX>
+__global__ __launch_bounds__(512, 1) void mx_ring_kernel(MxArgs g) {
+  constexpr int MI = 8;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wid >> 2, wn = wid & 3;
+  const int tiles_n = (g.N + 255) / 256, items = (g.M + 255) / 256 * tiles_n;
+  const int q8 = items >> 3, r8 = items & 7, xcd = blockIdx.x & 7;
+  const int tile = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (blockIdx.x >> 3);
+  const int m0 = tile / tiles_n * 256, n0 = tile % tiles_n * 256;
+  const uint32_t smem0 = (uint32_t)(uintptr_t)(VPT_LDS char*)smem;
+  const int nk = g.steps, r = lane & 15, blk = lane >> 4;
+  // v_perm selectors: byte blk of one dword into byte 0 (2), of the next into byte 1 (3), zeros elsewhere
+  const uint32_t sel_lo = 0x0c0c0400u + blk * 0x0101u, sel_hi = 0x04000c0cu + blk * 0x01010000u;
+  uint32_t va[2], vb[2];  // rows past the edge: the last one (its results are not stored)
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    va[i] = tile_voff<true, 256, 8>(g.lda >> 1, m0, g.M, RBK, wid, lane, i);
+    const int p = (wid * 2 + i) * 16 + (lane >> 2), row = (p & ~63) | mx_wrow(p & 63);
+    vb[i] = (uint32_t)(min(row, g.N - 1 - n0) * (int)g.ldb + ((lane & 3) ^ (((p >> 2) & 1) << 1)) * 16);
+  }
+  // scales: waves 0-3 fetch A's rows, 4-7 B's
+  const uint32_t vs = wid < 4 ? (uint32_t)(min(wid * 64 + lane, g.M - 1 - m0) * (int)g.ldas)
+                              : (uint32_t)(min((wid - 4) * 64 + mx_wrow(lane), g.N - 1 - n0) * (int)g.ldbs);
+  const uint8_t* sbase = wid < 4 ? g.AS + (long)m0 * g.ldas : g.BS + (long)n0 * g.ldbs;
+  const uint32_t ls = __builtin_amdgcn_readfirstlane(smem0 + MXR_ST * MXR_STG + wid * 1024);
+
+  float bias[2][8];
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int c = n0 + wn * 64 + q * 32 + blk * 8 + e;
+      bias[q][e] = g.bias && c < g.N ? bf2f(g.bias[c]) : 0.f;
+      asm volatile("" : "+v"(bias[q][e]));  // in registers before the first DMA
+    }
+  uint32_t sa[MI], sb[4];
+#pragma unroll
+  for (int i = 0; i < MI; ++i) sa[i] = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sb[j] = 0;
+  if (nk < 4) {  // no 16 bytes of scales in a row: straight into registers
+    for (int t = 0; t < nk; ++t) {
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+        sa[i] |= (uint32_t)g.AS[(long)min(m0 + wm * 128 + i * 16 + r, g.M - 1) * g.ldas + t * 4 + blk] << (8 * t);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        sb[j] |= (uint32_t)g.BS[(long)min(n0 + wn * 64 + mx_wrow(j * 16 + r), g.N - 1) * g.ldbs + t * 4 + blk] << (8 * t);
+    }
+  } else {
+    glds16(uniform_ptr(sbase), vs, ls);
+  }
+  floatx4 acc[MI][4];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+  for (int t = 0; t < 3 && t < nk; ++t) mxr_issue(g, va, vb, m0, n0, t, smem0, wid);
+  wait_younger(nk - 1);  // step 0 (and the scales) landed: the younger steps' 4 pieces each may fly
+  raw_barrier();
+  if (wid >= 4) bare_barrier();
+
+  auto step = [&](int kt, auto S_) {
+    constexpr int S = decltype(S_)::value;
+    const bool fetch = S == 1 && kt + 3 < nk;  // a last group of fewer than 4 steps' scales ends with the row
+    if (fetch) glds16(uniform_ptr(sbase + min(4 * (kt + 3), 4 * nk - 16)), vs, ls);
+    if (kt + 3 < nk) mxr_issue(g, va, vb, m0, n0, kt + 3, smem0, wid);
+    const char* st = smem + (kt % MXR_ST) * MXR_STG;
+    if (S == 0 && nk >= 4) {
+      const char* sc = smem + MXR_ST * MXR_STG;
+      const int rem = nk - kt, first = rem < 4 ? 4 - rem : 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sb[j] = mx_scale4(sc + 4096 + (wn * 64 + j * 16 + r) * 16, sel_lo, sel_hi, first);
+#pragma unroll
+      for (int i = 0; i < MI; ++i) sa[i] = mx_scale4(sc + (wm * 128 + i * 16 + r) * 16, sel_lo, sel_hi, first);
+    }
+    uint4 af[MI], bf[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) bf[j] = *reinterpret_cast<const uint4*>(st + 16384 + kmaj32_off(wn * 64 + j * 16 + r, blk));
+#pragma unroll
+    for (int i = 0; i < MI; ++i) af[i] = *reinterpret_cast<const uint4*>(st + kmaj32_off(wm * 128 + i * 16 + r, blk));
+    // this wave's pieces of step kt + 1 landed; steps kt + 2, kt + 3 (4 pieces each) and a scale piece issued at S = 1 fly
+    const bool scale_flies = (S == 1 && fetch) || (S == 2 && kt + 2 < nk);
+    if (kt + 3 < nk) {
+      if (scale_flies) asm volatile("s_waitcnt vmcnt(9)" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    } else if (kt + 2 < nk) {
+      if (scale_flies) asm volatile("s_waitcnt vmcnt(5)" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    raw_barrier();
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = mx_mfma_at<S>(bf[j], af[i], acc[i][j], sb[j], sa[i]);
+    __builtin_amdgcn_s_setprio(0);
+    bare_barrier();
+  };
+  for (int kt = 0; kt < nk; kt += 4) {
+    step(kt, std::integral_constant<int, 0>{});
+    if (kt + 1 < nk) step(kt + 1, std::integral_constant<int, 1>{});
+    if (kt + 2 < nk) step(kt + 2, std::integral_constant<int, 2>{});
+    if (kt + 3 < nk) step(kt + 3, std::integral_constant<int, 3>{});
+  }
+  if (wid < 4) bare_barrier();
+  mx_epilogue<VEC, AUX, MI, 2>(g, acc, lane, m0, n0, wm * 128, wn * 64, bias);
 }
 
 // ---- few rows: 16 MI rows x 16 columns per block, its 4 waves share the steps along K --------------------------------
@@ -554,7 +712,11 @@ int mx_check_product(const void* b_codes, long ldb, const void* b_scales, long l
   return VPT_OK;
 }
 
-constexpr int kMxSkinnyRows = 64;
+// Cache policy of the tile kernels' 16-byte stores (buffer instruction aux bits): sc1 (16: the line leaves the XCD's L2, which
+// the weight's rows keep) where the output fits the 256-MB cache, nt (2) where it does not. Measured (default / sc1 / nt):
+// 17568 x 2304 x 768 32.0 / 30.2 / 34.7 us, 24000 x 5120 x 768 (246 MB) - / 88.7 / 93.5, 33360 x 4096 x 768 (273 MB)
+// 124 / 109 / 93, 33360 x 4096 x 1536 - / 202 / 147.
+constexpr int kMxKeep = 16, kMxStream = 2;
 
 template <int MI>
 void mx_skinny_launch(const MxArgs& g, hipStream_t s) {
@@ -565,7 +727,9 @@ void mx_skinny_launch(const MxArgs& g, hipStream_t s) {
 // The product of checked arguments.
 void mx_product(const MxArgs& g, hipStream_t st) {
   const long tiles = ((g.M + 127L) / 128) * ((g.N + 127L) / 128);
-  if (g.M <= kMxSkinnyRows) {
+  // Few rows: also while blocks of 64 rows x 16 columns do not outnumber the CUs (65 x 1280 x 5120 13.6 us against 19.8 of the
+  // 128 x 128 tiles, 192 rows 13.9 : 20.1, 256 rows, 320 blocks, 24.6 : 20.3; 384 x 640 x 2048 7.7 : 10.2, 512 rows 11.6 : 10.2).
+  if (g.M <= 64 || ((g.M + 63L) / 64) * ((g.N + 15L) / 16) <= 256) {
     if (g.M <= 16) mx_skinny_launch<1>(g, st);
     else if (g.M <= 32) mx_skinny_launch<2>(g, st);
     else mx_skinny_launch<4>(g, st);
@@ -573,19 +737,34 @@ void mx_product(const MxArgs& g, hipStream_t st) {
   }
   // the tile kernels keep 32-bit offsets within a tile of at most 256 rows
   const long es = g.f32out ? 4 : 2, far = 1L << 22;
-  if (g.lda >= far || g.ldb >= far || g.ldas >= far || g.ldbs >= far) {
+  if (g.lda >= far || g.ldb >= far || g.ldas >= far || g.ldbs >= far || g.ldc * es >= far || (g.resid && g.ldr * 2 >= far)) {
     hipLaunchKernelGGL(mx_gemm_kernel, dim3((unsigned)tiles), dim3(256), 0, st, g);
     return;
   }
   const bool vec = g.N % 8 == 0 && aligned(g.C, 16) && g.ldc * es % 16 == 0 &&
                    (!g.resid || (aligned(g.resid, 16) && g.ldr % 8 == 0));
-  const long tiles256 = ((g.M + 255L) / 256) * ((g.N + 127L) / 128);
-  if (tiles256 >= 512) {
-    if (vec) hipLaunchKernelGGL((mx_tile_kernel<256, true>), dim3((unsigned)tiles256), dim3(256), mx_lds<256>(), st, g);
-    else hipLaunchKernelGGL((mx_tile_kernel<256, false>), dim3((unsigned)tiles256), dim3(256), mx_lds<256>(), st, g);
+  const bool stream = (long)g.M * g.N * es >= 256L << 20;
+  const long tiles256 = ((g.M + 255L) / 256) * ((g.N + 127L) / 128), tiles2 = ((g.M + 255L) / 256) * ((g.N + 255L) / 256);
+  // A step of a round of 256 x 256 tiles (one per CU) takes 1.02 us, of 256 x 128 tiles (two per CU) 1.27 us, whose blocks
+  // overlap their ends and waste less of a last round; short reductions are ends for the most part. Measured, 256 x 256 :
+  // 256 x 128: 4096^3 38.5 : 44.1 us, 8448 x 1280 x 5120 40.4 : 48.6, 33360 x 4096 x 3840 316 : 353, 8192^3 294 : 335; but
+  // 16384 x 1280 x 5120 (1.25 rounds) 82.8 : 76.8, 16384 x 2560 x 2560 74.5 : 68.7, 33360 x 4096 x 768 116 : 93.
+  const long rounds = (tiles2 + 255) / 256;
+  if (g.steps >= 24 && tiles2 > 128 && rounds * 102 < tiles2 * 127 / 256 + 20) {
+    const dim3 grid((unsigned)tiles2);
+    if (!vec) hipLaunchKernelGGL((mx_ring_kernel<false, 0>), grid, dim3(512), mx_ring_lds(), st, g);
+    else if (stream) hipLaunchKernelGGL((mx_ring_kernel<true, kMxStream>), grid, dim3(512), mx_ring_lds(), st, g);
+    else hipLaunchKernelGGL((mx_ring_kernel<true, kMxKeep>), grid, dim3(512), mx_ring_lds(), st, g);
+  } else if (tiles256 >= 768) {  // 1.5 rounds. 256 : 128 rows per tile: 33360 x 768 x 2048 (786) 40.4 : 42.7 us, 17568 x 2304 x
+                                 // 768 30.2 : 32.0; 8440 x 4096 x 768 29.7 : 27.7, 4224 x 1280 x 5120 (170) 30.5 : 29.4
+    const dim3 grid((unsigned)tiles256);
+    if (!vec) hipLaunchKernelGGL((mx_tile_kernel<256, false, 0>), grid, dim3(256), mx_lds<256>(), st, g);
+    else if (stream) hipLaunchKernelGGL((mx_tile_kernel<256, true, kMxStream>), grid, dim3(256), mx_lds<256>(), st, g);
+    else hipLaunchKernelGGL((mx_tile_kernel<256, true, kMxKeep>), grid, dim3(256), mx_lds<256>(), st, g);
   } else {
-    if (vec) hipLaunchKernelGGL((mx_tile_kernel<128, true>), dim3((unsigned)tiles), dim3(256), mx_lds<128>(), st, g);
-    else hipLaunchKernelGGL((mx_tile_kernel<128, false>), dim3((unsigned)tiles), dim3(256), mx_lds<128>(), st, g);
+    const dim3 grid((unsigned)tiles);
+    if (!vec) hipLaunchKernelGGL((mx_tile_kernel<128, false, 0>), grid, dim3(256), mx_lds<128>(), st, g);
+    else hipLaunchKernelGGL((mx_tile_kernel<128, true, kMxKeep>), grid, dim3(256), mx_lds<128>(), st, g);
   }
 }
 
