@@ -1281,6 +1281,16 @@ def _raw_stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+def _enqueue(dev: int, op: str, work: float, name: str, *args):
+    """One entry point on the current stream of device `dev`; `op` and `work` as in _launch."""
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return _enqueue(dev, op, work, name, *args)
+    if op in PROBES:
+        return PROBES[op].record(work, lambda: call(name, *args, _raw_stream(dev)))
+    return call(name, *args, _raw_stream(dev))
+
+
 def _need(cond: bool, msg: str):
     if not cond:
         raise ValueError(msg)
@@ -1301,7 +1311,7 @@ def _rows2d(t, fn: str, arg: str, dtypes, shape=None, align: int = 1):
     bytes."""
     sh = t.shape
     if (t.dtype in dtypes and (len(sh) == 2 if shape is None else sh == shape) and t.is_contiguous()
-            and (align == 1 or t.data_ptr() % align == 0 and (sh[0] <= 1 or sh[1] * t.element_size() % align == 0))):
+            and (align == 1 or not (t.data_ptr() % align or sh[0] > 1 and sh[1] * t.element_size() % align))):
         return
     _need(t.dtype in dtypes, f"{fn}: {arg}: dtype {t.dtype}, expected one of {[str(d) for d in dtypes]}")
     _need(t.dim() == 2 and (shape is None or tuple(t.shape) == tuple(shape)),
@@ -1313,8 +1323,7 @@ def _rows2d(t, fn: str, arg: str, dtypes, shape=None, align: int = 1):
 
 
 def _vec1d(t, fn: str, arg: str, dtype, n: int, align: int = 1):
-    sh = t.shape
-    if not (t.dtype == dtype and len(sh) == 1 and sh[0] == n and (n <= 1 or t.stride(0) == 1)):
+    if t.dtype is not dtype or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{fn}: {arg}: a contiguous {dtype} [{n}] tensor expected, got {t.dtype} {tuple(t.shape)}")
     if align > 1 and t.data_ptr() % align:
         raise ValueError(f"{fn}: {arg} at a multiple of {align} bytes")
@@ -1367,10 +1376,8 @@ def mxfp4_quantize(x, codes=None, scales=None):
     dev = _gpu("mxfp4_quantize", x, codes, scales)
     if M == 0:
         return codes, scales
-    with _on(dev):
-        _launch("mxfp4_quantize", M * K * (x.element_size() + 17 / 32),
-                lambda: call("vpt_mxfp4_quantize", x.data_ptr(), _MX_DTYPES[x.dtype], _ld(x), M, K, codes.data_ptr(),
-                             _ld(codes), scales.data_ptr(), _ld(scales), _raw_stream(dev)))
+    _enqueue(dev, "mxfp4_quantize", M * K * (x.element_size() + 17 / 32), "vpt_mxfp4_quantize", x.data_ptr(),
+             _MX_DTYPES[x.dtype], _ld(x), M, K, codes.data_ptr(), _ld(codes), scales.data_ptr(), _ld(scales))
     return codes, scales
 
 
@@ -1387,10 +1394,8 @@ def mxfp4_dequantize(codes, scales, K: int, out=None, dtype=BF16):
     dev = _gpu("mxfp4_dequantize", codes, scales, out)
     if M == 0:
         return out
-    with _on(dev):
-        _launch("mxfp4_dequantize", M * K * (out.element_size() + 17 / 32),
-                lambda: call("vpt_mxfp4_dequantize", codes.data_ptr(), _ld(codes), scales.data_ptr(), _ld(scales), M, K,
-                             out.data_ptr(), _ld(out), int(out.dtype == F32), _raw_stream(dev)))
+    _enqueue(dev, "mxfp4_dequantize", M * K * (out.element_size() + 17 / 32), "vpt_mxfp4_dequantize", codes.data_ptr(),
+             _ld(codes), scales.data_ptr(), _ld(scales), M, K, out.data_ptr(), _ld(out), int(out.dtype == F32))
     return out
 
 
@@ -1418,11 +1423,9 @@ def gemm_mxfp4(a_codes, a_scales, w, out=None, *, bias=None, resid=None, out_dty
     dev = _gpu("gemm_mxfp4", a_codes, a_scales, w.codes, w.scales, out, bias, resid)
     if M == 0:
         return out
-    with _on(dev):
-        _launch("gemm_mxfp4", 2.0 * M * N * K,
-                lambda: call("vpt_gemm_mxfp4", a_codes.data_ptr(), _ld(a_codes), a_scales.data_ptr(), _ld(a_scales),
-                             w.codes.data_ptr(), _ld(w.codes), w.scales.data_ptr(), _ld(w.scales), out.data_ptr(),
-                             _ld(out), M, N, K, _p(bias), *_ptr_ld(resid), int(out.dtype == F32), _raw_stream(dev)))
+    _enqueue(dev, "gemm_mxfp4", 2.0 * M * N * K, "vpt_gemm_mxfp4", a_codes.data_ptr(), _ld(a_codes),
+             a_scales.data_ptr(), _ld(a_scales), w.codes.data_ptr(), _ld(w.codes), w.scales.data_ptr(), _ld(w.scales),
+             out.data_ptr(), _ld(out), M, N, K, _p(bias), *_ptr_ld(resid), int(out.dtype == F32))
     return out
 
 
@@ -1441,11 +1444,9 @@ def linear_mxfp4(x, w, bias=None, resid=None, out=None, out_dtype=BF16):
         return out
     n = call("vpt_linear_mxfp4_workspace", M, K)
     ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-    with _on(dev):
-        _launch("linear_mxfp4", 2.0 * M * N * K,
-                lambda: call("vpt_linear_mxfp4", x.data_ptr(), _MX_DTYPES[x.dtype], _ld(x), w.codes.data_ptr(),
-                             _ld(w.codes), w.scales.data_ptr(), _ld(w.scales), out.data_ptr(), _ld(out), M, N, K, _p(bias),
-                             *_ptr_ld(resid), int(out.dtype == F32), _p(ws), _raw_stream(dev)))
+    _enqueue(dev, "linear_mxfp4", 2.0 * M * N * K, "vpt_linear_mxfp4", x.data_ptr(), _MX_DTYPES[x.dtype], _ld(x),
+             w.codes.data_ptr(), _ld(w.codes), w.scales.data_ptr(), _ld(w.scales), out.data_ptr(), _ld(out), M, N, K,
+             _p(bias), *_ptr_ld(resid), int(out.dtype == F32), _p(ws))
     return out
 
 
@@ -1469,7 +1470,7 @@ def linear_mxfp4_dgrad(dy, w, out=None):
     if M == 0:
         return out
     dense = lambda t: t if M > 1 else t.as_strided(t.shape, (t.shape[1], 1))  # noqa: E731 (one row: any stride)
-    with _on(dev):
+    with _on(dev):  # linear_dgrad launches on the current device
         linear_dgrad(dense(dy), mxfp4_dequantize(w.codes, w.scales, K), out=dense(out))
     return out
 
@@ -1546,12 +1547,10 @@ def gated_norm_fwd(h, x, *, w_post=None, w_pre=None, gate=None, scale=None, shif
     rstd_post = None if w_post is None else torch.empty(M, dtype=F32, device=x.device)
     rstd_pre = None if w_pre is None else torch.empty(M, dtype=F32, device=x.device)
     if M:
-        with _on(dev):
-            _launch("gated_norm_fwd", M * D * (2 + 2 * x.element_size() + (0 if y is None else 2)),
-                    lambda: call("vpt_gated_norm_fwd", h.data_ptr(), _ld(h), x.data_ptr(), int(x.dtype == F32), _ld(x),
-                                 _p(w_post), _p(w_pre), *_gn_vec(gate), *_gn_vec(scale), *_gn_vec(shift),
-                                 x_out.data_ptr(), _ld(x_out), *_ptr_ld(y), _p(rstd_post), _p(rstd_pre), groups,
-                                 M // groups, D, float(resid_scale), float(eps), _raw_stream(dev)))
+        _enqueue(dev, "gated_norm_fwd", M * D * (2 + 2 * x.element_size() + (0 if y is None else 2)),
+                 "vpt_gated_norm_fwd", h.data_ptr(), _ld(h), x.data_ptr(), int(x.dtype == F32), _ld(x), _p(w_post),
+                 _p(w_pre), *_gn_vec(gate), *_gn_vec(scale), *_gn_vec(shift), x_out.data_ptr(), _ld(x_out), *_ptr_ld(y),
+                 _p(rstd_post), _p(rstd_pre), groups, M // groups, D, float(resid_scale), float(eps))
     return x_out, y, rstd_post, rstd_pre
 
 
@@ -1597,16 +1596,13 @@ def gated_norm_bwd(dy, dx_new, h, x_new, rstd_post, rstd_pre, *, w_post=None, w_
     make = torch.empty if M else torch.zeros
     grad = [None if v is None else make(v.shape, dtype=F32, device=h.device) for v in (w_post, w_pre, gate, scale, shift)]
     if M:
-        with _on(dev):
-            sums = any(g is not None for g in grad)
-            ws = torch.empty(call("vpt_gated_norm_bwd_workspace", groups, M // groups, D), dtype=torch.uint8,
-                             device=h.device) if sums else None
-            e = h.element_size() * 2 + (dx.element_size() * 3 + 2 if w_pre is not None else dx.element_size())
-            _launch("gated_norm_bwd", M * D * e,
-                    lambda: call("vpt_gated_norm_bwd", *_ptr_ld(dy), *_ptr_ld(dx_new), h.data_ptr(), _ld(h),
-                                 _p(x_new), int(kind == F32), 0 if x_new is None else _ld(x_new), _p(rstd_post),
-                                 _p(rstd_pre), _p(w_post), _p(w_pre), *_gn_vec(gate), *_gn_vec(scale), *_gn_vec(shift),
-                                 dh.data_ptr(), _ld(dh), *(_ptr_ld(dx) if w_pre is not None else (None, 0)),
-                                 *(_p(g) for g in grad), _p(ws), groups, M // groups, D,
-                                 float(resid_scale), _raw_stream(dev)))
+        sums = any(g is not None for g in grad)
+        ws = torch.empty(call("vpt_gated_norm_bwd_workspace", groups, M // groups, D), dtype=torch.uint8,
+                         device=h.device) if sums else None
+        e = h.element_size() * 2 + (dx.element_size() * 3 + 2 if w_pre is not None else dx.element_size())
+        _enqueue(dev, "gated_norm_bwd", M * D * e, "vpt_gated_norm_bwd", *_ptr_ld(dy), *_ptr_ld(dx_new), h.data_ptr(), _ld(h),
+                 _p(x_new), int(kind == F32), 0 if x_new is None else _ld(x_new), _p(rstd_post), _p(rstd_pre), _p(w_post),
+                 _p(w_pre), *_gn_vec(gate), *_gn_vec(scale), *_gn_vec(shift), dh.data_ptr(), _ld(dh),
+                 *(_ptr_ld(dx) if w_pre is not None else (None, 0)), *(_p(g) for g in grad), _p(ws), groups, M // groups, D,
+                 float(resid_scale))
     return GatedNormGrads(dh, dx, *grad)
