@@ -20,6 +20,7 @@ import contextlib
 import torch
 
 from . import ops
+from .mxfp4 import MXFP4Weight
 
 BF16 = torch.bfloat16
 F32 = torch.float32
@@ -115,6 +116,14 @@ def _dequant_scratch(base: "NF4Weight", device) -> torch.Tensor:
     return base.dequantize(buf[:base.numel].view(base.shape))
 
 
+def dequant_into(pairs):
+    """[(base, bf16 out)]: the NF4 bases in one launch per 16 (vpt_nf4_dequant_batch), MXFP4 bases one by one."""
+    ops.nf4_dequant_batch([(b, o) for b, o in pairs if isinstance(b, NF4Weight)])
+    for b, o in pairs:
+        if isinstance(b, MXFP4Weight):
+            b.dequantize(o)
+
+
 def dequant_bases(lins: dict, targets, device) -> dict:
     """{target: bf16 base} for a block's LoRA targets about to run: "dequant" mode dequantises all of them in ONE
     launch (vpt_nf4_dequant_batch) into a shared per-device scratch (stream-ordered reuse, block after block);
@@ -139,7 +148,7 @@ def dequant_bases(lins: dict, targets, device) -> dict:
         b = lins[t].base
         out[t] = buf[off:off + b.numel].view(b.shape)
         off += b.numel
-    ops.nf4_dequant_batch([(lins[t].base, out[t]) for t in ts])
+    dequant_into([(lins[t].base, out[t]) for t in ts])
     if ts[:3] == QKV:  # the three self-attention bases are side by side: the stacked [3 dim, dim] operand
         n = lins[QKV[0]].base.numel
         out["attn1.qkv"] = buf[:3 * n].view(3 * lins[QKV[0]].base.shape[0], lins[QKV[0]].base.shape[1])
@@ -156,7 +165,8 @@ def base_weight(base: "NF4Weight", mode: str, device) -> torch.Tensor:
 
 
 class LoRALinearNF4:
-    """a29. `down` [r, in], `up` [out, r] bf16 trainable (grads `g_down`, `g_up` f32); `base` NF4 [out, in].
+    """a29. `down` [r, in], `up` [out, r] bf16 trainable (grads `g_down`, `g_up` f32); `base` NF4 [out, in] (an NF4Weight), or
+    a vpt.mxfp4.MXFP4Weight in the "dequant" and "resident" modes (its bf16 values take the place of NF4's).
 
     forward  ds = bf16(s * x . down^T)            (one skinny GEMM, s = alpha / rank folded into its epilogue)
              y  = bf16(x . Wd^T + b + ds . up^T)  (vpt_gemm_bf16_lora on the dequantised base, or vpt_gemm_nf4
@@ -172,6 +182,8 @@ class LoRALinearNF4:
         self.base_mode = base_mode or DEFAULT_BASE_MODE
         if self.base_mode not in BASE_MODES:
             raise ValueError(f"base_mode must be one of {BASE_MODES}")
+        if self.base_mode == "inline" and not isinstance(base, NF4Weight):
+            raise ValueError("base_mode \"inline\" dequantises NF4 inside the GEMM: an NF4Weight only")
         self.down, self.up = down.to(BF16).contiguous(), up.to(BF16).contiguous()
         self.scale = alpha / rank
         self.g_down = torch.zeros(self.down.shape, dtype=F32, device=self.down.device)
@@ -330,8 +342,9 @@ QKV = TARGETS[:3]
 
 class SDXLTransformerBlock:
     """a30. Weights from a reference-named state dict: `<target>.linear.weight` given either as an NF4
-    state ({packed, qabsmax, absmax2, code2, offset, shape}) or as a dense tensor (quantised on load),
-    `<target>.linear.bias`, `<target>.lora_down.weight`, `<target>.lora_up.weight`, `norm{1,2,3}.{weight,bias}`."""
+    state ({packed, qabsmax, absmax2, code2, offset, shape}), as a dense tensor (quantised on load) or as a
+    vpt.mxfp4.MXFP4Weight, `<target>.linear.bias`, `<target>.lora_down.weight`, `<target>.lora_up.weight`,
+    `norm{1,2,3}.{weight,bias}`."""
 
     def __init__(self, dim: int, heads: int, context_dim: int, rank: int, alpha: float, sd: dict, code2=None,
                  device="cuda", head_dim: int = 64):
@@ -342,7 +355,9 @@ class SDXLTransformerBlock:
         self.device = device
         self.lin = {}
         for t in TARGETS:
-            base = _nf4_or_dense(sd[f"{t}.linear.weight"], code2, device)
+            base = sd[f"{t}.linear.weight"]
+            if not isinstance(base, MXFP4Weight):
+                base = _nf4_or_dense(base, code2, device)
             b = sd.get(f"{t}.linear.bias")
             self.lin[t] = LoRALinearNF4(base, None if b is None else b.to(device, BF16).contiguous(),
                                         sd[f"{t}.lora_down.weight"].to(device), sd[f"{t}.lora_up.weight"].to(device),

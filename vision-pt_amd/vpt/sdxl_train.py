@@ -33,7 +33,7 @@ import torch
 
 from . import ops
 from .optim import RAdamScheduleFreeFlat
-from .sdxl import TARGETS, SDXLSpatialTransformer, dynamic_map, lora_side_scope
+from .sdxl import TARGETS, SDXLSpatialTransformer, dequant_into, dynamic_map, lora_side_scope
 
 BF16, F32 = torch.bfloat16, torch.float32
 
@@ -196,7 +196,7 @@ class SDXLStacksQLoRA:
                     self._kv_resident = {**getattr(self, "_kv_resident", {}), w: W}
             else:
                 W = ops.workspace(self.device, f"kv_base{w}", G * w * cd, BF16).view(G * w, cd)
-                ops.nf4_dequant_batch([(l.base, W[i * w:(i + 1) * w]) for i, l in enumerate(group)])
+                dequant_into([(l.base, W[i * w:(i + 1) * w]) for i, l in enumerate(group)])
             out = ops.workspace(self.device, f"kv_out{w}", M * G * w, BF16).view(M, G * w)
             ops.gemm_lora_stacked(ctx, W, ds[:, c0:c0 + G * r], ups, w, out)
             for i, l in enumerate(group):
