@@ -372,3 +372,36 @@ def test_linear_large(m, M, N, K):
     x, wt, b, r, w, y = product(m, M, N, K, seed=K, out_dtype=F32 if K == 300 else BF16)
     close(y, x, wt, b, r)
     assert torch.equal(m[0].linear_mxfp4(x, w, bias=b, resid=r, out_dtype=y.dtype), y)
+
+
+@pytest.mark.parametrize("M,N,K", [(8200, 3080, 200), (8200, 3080, 640), (8200, 3073, 640), (33000, 4100, 128), (33000, 4104, 128),
+                                   (33000, 4104, 3100), (70000, 2000, 520)])
+def test_linear_sampled(m, M, N, K):
+    """Large results, also past what the cache holds, checked on rows of every part of them."""
+    ops, mxfp4 = m
+    x = rnd(512, K, seed=K, spread=1.0).repeat(-(-M // 512), 1)[:M].contiguous()
+    wt, b, r = rnd(N, K, dtype=F32, seed=1), rnd(N, seed=2), rnd(M, N, seed=3)
+    y = ops.linear_mxfp4(x, mxfp4.MXFP4Weight.quantize(wt), bias=b, resid=r)
+    at = torch.tensor(sorted({0, 1, 15, 16, 127, 128, 255, 256, 4095, M // 2, M // 2 + 77, M - 257, M - 130, M - 17, M - 1}), device=DEV)
+    close(y[at], x[at], wt, b, r[at])
+    part = ops.linear_mxfp4(x[:512], mxfp4.MXFP4Weight.quantize(wt), bias=b).double()  # every row: the same product, other bits of r
+    for lo in range(0, M, 512):
+        n = min(512, M - lo)
+        d = (y[lo:lo + n].double() - r[lo:lo + n].double() - part[:n]).abs()
+        assert (d <= 2.0 ** -7 * (part[:n].abs() + r[lo:lo + n].double().abs()) + 1e-3).all()
+
+
+@pytest.mark.parametrize("M", [1, 3, 8, 16, 17, 40, 64, 65, 100, 300, 1000])
+@pytest.mark.parametrize("K", [96, 768, 2048])
+def test_linear_is_quantize_and_gemm(m, M, K):
+    ops, mxfp4 = m
+    x, w, b = rnd(M, K, seed=M), mxfp4.MXFP4Weight.quantize(rnd(200, K, seed=K)), rnd(200, seed=5)
+    assert torch.equal(ops.linear_mxfp4(x, w, bias=b), ops.gemm_mxfp4(*ops.mxfp4_quantize(x), w, bias=b))
+
+
+def test_dgrad_refuses_far_rows(m):
+    ops, mxfp4 = m
+    w = mxfp4.MXFP4Weight.quantize(rnd(16, 64))
+    dy = torch.zeros(2, 1 << 23, dtype=BF16, device=DEV)[:, :16]
+    with pytest.raises(ValueError, match="apart"):
+        ops.linear_mxfp4_dgrad(dy, w)

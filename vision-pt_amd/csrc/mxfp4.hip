@@ -559,6 +559,21 @@ __global__ __launch_bounds__(256) void mx_skinny_kernel(MxArgs g, MxX x) {
   const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (16 * MI);
   const int pitch = 64 * g.steps + 16;
   char* lscale = smem + (long)g.M * pitch;
+  const int r = lane & 15, blk = lane >> 4;
+  const long wrow = min(n0 + r, g.N - 1);  // rows past the edge: the last one (its results are not stored)
+  const uint8_t* wb = g.B + wrow * g.ldb + blk * 16;
+  const uint8_t* ws = g.BS + wrow * g.ldbs + blk;
+  uint4 bf[kMxSkinnyLoads];
+  uint32_t sb[kMxSkinnyLoads];
+  auto load_w = [&](int t0) {
+#pragma unroll
+    for (int u = 0; u < kMxSkinnyLoads; ++u) {
+      const int t = t0 + 4 * u;  // wave-uniform
+      if (t >= g.steps) break;
+      bf[u] = *reinterpret_cast<const uint4*>(wb + (long)t * 64);
+      sb[u] = ws[(long)t * 4];
+    }
+  };
   if (FUSE) {
     const int nch = 16 * g.steps, total = g.M * nch;
     for (int idx = tid; idx < total; idx += 256) {  // total % 16 == 0: the four lanes of a block stay together
@@ -576,10 +591,6 @@ __global__ __launch_bounds__(256) void mx_skinny_kernel(MxArgs g, MxX x) {
     }
     __syncthreads();
   }
-  const int r = lane & 15, blk = lane >> 4;
-  const long wrow = min(n0 + r, g.N - 1);  // rows past the edge: the last one (its results are not stored)
-  const uint8_t* wb = g.B + wrow * g.ldb + blk * 16;
-  const uint8_t* ws = g.BS + wrow * g.ldbs + blk;
   const uint8_t* ab[MI];
   const uint8_t* as[MI];
 #pragma unroll
@@ -592,14 +603,7 @@ __global__ __launch_bounds__(256) void mx_skinny_kernel(MxArgs g, MxX x) {
 #pragma unroll
   for (int i = 0; i < MI; ++i) acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
   for (int t0 = wid; t0 < g.steps; t0 += 4 * kMxSkinnyLoads) {
-    uint4 bf[kMxSkinnyLoads];
-    uint32_t sb[kMxSkinnyLoads];
-#pragma unroll
-    for (int u = 0; u < kMxSkinnyLoads; ++u) {
-      const int t = min(t0 + 4 * u, g.steps - 1);  // past the end: loaded, not used
-      bf[u] = *reinterpret_cast<const uint4*>(wb + (long)t * 64);
-      sb[u] = ws[(long)t * 4];
-    }
+    load_w(t0);
 #pragma unroll
     for (int u = 0; u < kMxSkinnyLoads; ++u) {
       const int t = t0 + 4 * u;  // wave-uniform
@@ -768,10 +772,12 @@ void mx_product(const MxArgs& g, hipStream_t st) {
   }
 }
 
-// LDS of the fused form, 0 where it is not taken.
+// LDS of the fused form, 0 where it is not taken: up to 16384 values of x, which every block quantises anew. Fused : two
+// launches, in a graph, K x M (N = 2304): 768 x 1 2.5 : 4.0 us, 768 x 16 4.5 : 4.5, 2048 x 8 5.9 : 5.4, 2048 x 16 8.9 : 5.8,
+// 5120 x 2 6.0 : 7.2, 5120 x 4 7.9 : 7.4 (outside a graph the second launch costs about 4 us of the host more).
 size_t mx_fused_lds(long M, int K) {
-  const long steps = (K + 127) / 128, bytes = M * (68 * steps + 16);
-  return M <= 16 && bytes <= 48 * 1024 ? (size_t)bytes : 0;
+  const long steps = (K + 127) / 128;
+  return M <= 16 && M * steps <= 128 ? (size_t)(M * (68 * steps + 16)) : 0;
 }
 
 template <int T>

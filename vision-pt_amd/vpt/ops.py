@@ -1453,7 +1453,7 @@ def linear_mxfp4(x, w, bias=None, resid=None, out=None, out_dtype=BF16):
 def linear_mxfp4_dgrad(dy, w, out=None):
     """dx = dy . W: the input gradient of linear_mxfp4, straight through the rounding of its input (dy [M, N] bf16, dx
     [M, K] bf16). W is dequantised to bf16 (exact) and goes through the bf16 GEMM, whose rows start at multiples of 16
-    bytes: N % 8 == 0 and K % 8 == 0, and dy and out with such rows."""
+    bytes, less than 2^22 values apart: N % 8 == 0 and K % 8 == 0, and dy and out with such rows."""
     N, K = w.shape
     M = dy.shape[0]
     _rows2d(dy, "linear_mxfp4_dgrad", "dy", (BF16,))
@@ -1462,6 +1462,8 @@ def linear_mxfp4_dgrad(dy, w, out=None):
     if N % 8 or K % 8:
         raise ValueError(f"linear_mxfp4_dgrad: N and K multiples of 8, W {w.shape}")
     _rows2d(dy, "linear_mxfp4_dgrad", "dy", (BF16,), None, 16)
+    if _ld(dy) >= 1 << 22 or K >= 1 << 22 or out is not None and M > 1 and out.stride(0) >= 1 << 22:
+        raise ValueError("linear_mxfp4_dgrad: rows less than 2^22 values apart (the GEMM's tiles have 32-bit offsets)")
     if out is None:
         out = torch.empty(M, K, dtype=BF16, device=dy.device)
     else:
