@@ -405,3 +405,15 @@ def test_dgrad_refuses_far_rows(m):
     dy = torch.zeros(2, 1 << 23, dtype=BF16, device=DEV)[:, :16]
     with pytest.raises(ValueError, match="apart"):
         ops.linear_mxfp4_dgrad(dy, w)
+
+
+@pytest.mark.parametrize("M,N,K", [(300, 200, 300), (8200, 3080, 200), (4000, 4000, 3100)])
+@pytest.mark.parametrize("off", [0, 1, 2, 4])
+def test_bias_anywhere(m, M, N, K, off):
+    """A bias that starts at any place of its buffer, at every tile kernel, the buffer ending with it."""
+    ops, mxfp4 = m
+    x, w = rnd(M, K, seed=1), mxfp4.MXFP4Weight.quantize(rnd(N, K, seed=2))
+    b = rnd(N, seed=3)
+    at = torch.empty(off + N, dtype=BF16, device=DEV)[off:].copy_(b)
+    zero = ops.linear_mxfp4(x, w, out_dtype=F32)
+    assert torch.equal(ops.linear_mxfp4(x, w, bias=at, out_dtype=F32), zero + b.float())
