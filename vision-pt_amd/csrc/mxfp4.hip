@@ -82,7 +82,8 @@ __device__ __forceinline__ uint32_t mx_codes8(const float (&f)[8], uint32_t s) {
   return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(out, f[6] * inv, f[7] * inv, 1.f, 3);
 }
 
-// One thread per 8 values: four neighbouring lanes share a block. Bound by HBM: 2 (or 4) bytes in, 17 / 32 out per value.
+// One thread per 8 values: four neighbouring lanes share a block, its largest magnitude by two DPP exchanges. Bound by HBM:
+// 2 (or 4) bytes in, 17 / 32 out per value; 33360 x 2048 bf16 in 35 us, 4.9 TB/s (a 4-GB copy runs at 4.6).
 template <int T, bool VEC>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const void* __restrict__ x, long ldx, unsigned total,
                                                           unsigned nch, int K, uint8_t* __restrict__ codes, long ldc,
@@ -111,7 +112,7 @@ __device__ __forceinline__ float mx_unit(uint32_t s) {  // 2^(s - 127); NaN for 
   return __uint_as_float(s == 255u ? 0x7fc00000u : s ? s << 23 : 1u << 22);
 }
 
-// One thread per 8 values. VEC: K % 8 == 0 and 16-byte rows.
+// One thread per 8 values. VEC: K % 8 == 0 and 16-byte rows. Bound by HBM as the quantisation: 33360 x 2048 to bf16 in 34 us.
 template <bool F32OUT, bool VEC>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t* __restrict__ codes, long ldc,
                                                             const uint8_t* __restrict__ scales, long lds, unsigned total,
@@ -167,6 +168,10 @@ __device__ __forceinline__ floatx4 mx_mfma(uint4 a, uint4 b, floatx4 c, uint32_t
 // steps into registers at the first of them, and the next 4 steps' piece is fetched from the second on.
 // The product is taken transposed, W's fragment first, so that a lane holds 4 consecutive columns of one output row; W's rows
 // lie in LDS in an order (mx_wrow) that makes the columns of two fragments neighbours: 16-byte stores from registers.
+// What bounds it: 1.27 us per step of a CU's two blocks, of which the MFMAs need 0.6 at the 7.0 PFLOP/s that the instruction
+// reaches on random operands (9.8 on zeros); the rest is fragment reads (64 bytes a clock) and LDS-DMA, and for short
+// reductions the stores: 33360 x 4096 x 768 takes 98 us, 67 without its 273 MB of stores. 17568 x 2304 x 768 31 us,
+// 4224 x 1280 x 5120 (128-row tiles) 29 us.
 constexpr int MXST = 3;
 template <int TM> constexpr int mx_stage() { return (TM + 128) * 64; }               // 24 / 16 KB
 template <int TM> constexpr int mx_lds() { return MXST * mx_stage<TM>() + (TM + 128) * 16; }  // 78 / 52 KB
@@ -434,6 +439,8 @@ __global__ __launch_bounds__(256, 2) void mx_tile_kernel(MxArgs g) {
 // A stage is refilled in L_t, after both groups' L_t-1 closed with lgkmcnt(0) and a barrier; a step's pieces of all waves have
 // landed one barrier before the first group reads them. The scales' buffer (one, 16 bytes per row) is read in L_4c and
 // refilled from L_4c+1 on; its piece has landed where step 4c + 4's are waited for.
+// 1.02 us per step: 8192^3 in 294 us, 3.7 PFLOP/s. Wider waves (four of 128 x 128, a third less LDS reading, fragments a step
+// ahead in registers) took 1.16: one wave per SIMD leaves its waits uncovered.
 constexpr int MXR_ST = 4, MXR_STG = 512 * 64;
 constexpr int mx_ring_lds() { return MXR_ST * MXR_STG + 512 * 16; }  // 136 KB
 
@@ -552,7 +559,9 @@ __global__ __launch_bounds__(512, 1) void mx_ring_kernel(MxArgs g) {
 // ---- few rows: 16 MI rows x 16 columns per block, its 4 waves share the steps along K --------------------------------
 // With few rows the product is a pass over W: each wave takes every fourth 128-deep step, its 16 rows of W straight from
 // memory into registers (four steps' loads in flight), and the four partial sums meet in LDS in a fixed order. FUSE: the block
-// quantises its rows of x itself, into LDS (M <= 16; the same codes as mx_quantize_kernel), and saves a launch.
+// quantises its rows of x itself, into LDS (M <= 16; the same codes as mx_quantize_kernel), and saves a launch. One row
+// of 2304 x 768: 2.5 us in a graph; of 10240 x 5120: 10 us, 2.8 TB/s of codes, bound by the latency of its few loads in
+// flight (8 instead of 4 per wave, or the first ones before x is quantised, were slower).
 struct MxX {
   const void* x; long ldx;
   int K;
@@ -638,7 +647,8 @@ __global__ __launch_bounds__(256) void mx_skinny_kernel(MxArgs g, MxX x) {
   }
 }
 
-// 128 x 128 tile, 4 waves of 64 x 64, one 128-deep step at a time through LDS.
+// Rows too far apart for the tile kernels' 32-bit offsets: 128 x 128 tile, 4 waves of 64 x 64, one 128-deep step at a time
+// through LDS with 64-bit addresses (505 us where the tile kernels take 112 for x, quantised, of 33360 x 4096 x 768).
 __global__ __launch_bounds__(256) void mx_gemm_kernel(MxArgs g) {
   __shared__ __attribute__((aligned(16))) char as[128 * 64], bs[128 * 64];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, wm = wid >> 1, wn = wid & 1;

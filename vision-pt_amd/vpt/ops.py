@@ -1595,8 +1595,13 @@ def gated_norm_bwd(dy, dx_new, h, x_new, rstd_post, rstd_pre, *, w_post=None, w_
     else:
         _rows2d(dh, fn, "dh", _BF16, (M, D), 16)
     dev = _gpu("gated_norm_bwd", h, dy, dx_new, x_new, rstd_post, rstd_pre, w_post, w_pre, gate, scale, shift, dh, dx)
+    vecs = (w_post, w_pre, gate, scale, shift)
     make = torch.empty if M else torch.zeros
-    grad = [None if v is None else make(v.shape, dtype=F32, device=h.device) for v in (w_post, w_pre, gate, scale, shift)]
+    one = [v is not None and v.dim() == 1 for v in vecs]  # gradients of one shape share an allocation
+    ones = iter(make(sum(one), D, dtype=F32, device=h.device).unbind(0) if any(one) else ())
+    eachs = sum(v is not None for v in vecs) - sum(one)
+    eachs = iter(make(eachs, groups, D, dtype=F32, device=h.device).unbind(0) if eachs else ())
+    grad = [None if v is None else next(ones) if o else next(eachs) for v, o in zip(vecs, one)]
     if M:
         sums = any(g is not None for g in grad)
         ws = torch.empty(call("vpt_gated_norm_bwd_workspace", groups, M // groups, D), dtype=torch.uint8,
