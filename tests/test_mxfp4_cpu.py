@@ -116,7 +116,7 @@ def test_c_abi_refuses(m):
         assert lib.vpt_mxfp4_dequantize(*a) == 1, (i, v)
     ok_g = [p, 128, p, 8, p, 128, p, 8, p, 64, 4, 64, 256, p, p, 64, 0, None]
     for i, v in [(0, None), (1, 64), (1, 136), (2, None), (3, 4), (4, p + 8), (5, 120), (6, p + 1), (7, 6), (8, None), (8, q),
-                 (9, 63), (10, -1), (11, 0), (12, 0), (13, q), (14, q), (15, 63)]:
+                 (9, 63), (10, -1), (10, (1 << 30) + 1), (11, 0), (11, (1 << 30) + 1), (12, 0), (13, q), (14, q), (15, 63)]:
         a = list(ok_g)
         a[i] = v
         assert lib.vpt_gemm_mxfp4(*a) == 1, (i, v)

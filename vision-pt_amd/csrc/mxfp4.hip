@@ -195,8 +195,8 @@ __device__ __forceinline__ void mx_issue(const MxArgs& g, const MxOffs& o, int m
   const uint32_t lb = __builtin_amdgcn_readfirstlane(st + TM * 64 + wid * 2048);
   if constexpr (TM == 256) {
     glds_step(ab, bb, o.a[0], o.a[1], o.b[0], o.b[1], la, la + 1024, lb, lb + 1024);
-    glds16(ab, o.a[2], la + 2048);
-    glds16(ab, o.a[3], la + 3072);
+    glds16(ab, o.a[2], la + 2 * 1024);
+    glds16(ab, o.a[3], la + 3 * 1024);
   } else {
     glds_step(ab, bb, o.a[0], o.a[1], o.b[0], o.b[1], la, la + 1024, lb, lb + 1024);
   }
@@ -480,30 +480,15 @@ __global__ __launch_bounds__(512, 1) void mx_ring_kernel(MxArgs g) {
   float bias[2][8];
   mx_bias<VEC>(g, n0 + wn * 64 + blk * 8, bias);
   uint32_t sa[MI], sb[4];
-#pragma unroll
-  for (int i = 0; i < MI; ++i) sa[i] = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) sb[j] = 0;
-  if (nk < 4) {  // no 16 bytes of scales in a row: straight into registers
-    for (int t = 0; t < nk; ++t) {
-#pragma unroll
-      for (int i = 0; i < MI; ++i)
-        sa[i] |= (uint32_t)g.AS[(long)min(m0 + wm * 128 + i * 16 + r, g.M - 1) * g.ldas + t * 4 + blk] << (8 * t);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        sb[j] |= (uint32_t)g.BS[(long)min(n0 + wn * 64 + mx_wrow(j * 16 + r), g.N - 1) * g.ldbs + t * 4 + blk] << (8 * t);
-    }
-  } else {
-    glds16(uniform_ptr(sbase), vs, ls);
-  }
+  glds16(uniform_ptr(sbase), vs, ls);  // the host takes this kernel for 24 steps and more: every row has 16 bytes of scales
   floatx4 acc[MI][4];
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
 
-  for (int t = 0; t < 3 && t < nk; ++t) mxr_issue(g, va, vb, m0, n0, t, smem0, wid);
-  wait_younger(nk - 1);  // step 0 (and the scales) landed: the younger steps' 4 pieces each may fly
+  for (int t = 0; t < 3; ++t) mxr_issue(g, va, vb, m0, n0, t, smem0, wid);
+  wait_younger(2);  // step 0 and the scales landed: the two younger steps' 4 pieces each may fly
   raw_barrier();
   if (wid >= 4) bare_barrier();
 
@@ -513,7 +498,7 @@ __global__ __launch_bounds__(512, 1) void mx_ring_kernel(MxArgs g) {
     if (fetch) glds16(uniform_ptr(sbase + min(4 * (kt + 3), 4 * nk - 16)), vs, ls);
     if (kt + 3 < nk) mxr_issue(g, va, vb, m0, n0, kt + 3, smem0, wid);
     const char* st = smem + (kt % MXR_ST) * MXR_STG;
-    if (S == 0 && nk >= 4) {
+    if (S == 0) {
       const char* sc = smem + MXR_ST * MXR_STG;
       const int rem = nk - kt, first = rem < 4 ? 4 - rem : 0;
 #pragma unroll
@@ -717,7 +702,6 @@ void mx_quantize_launch(const void* x, long ldx, long rows, unsigned nch, int K,
                      codes, ldc, scales, lds);
 }
 
-
 // W, the output, bias and residual of a product.
 int mx_check_product(const void* b_codes, long ldb, const void* b_scales, long ldbs, const void* C, long ldc, int M, int N, int K,
                      const void* bias, const void* resid, long ldr, int f32_out) {
@@ -739,6 +723,7 @@ int mx_check_product(const void* b_codes, long ldb, const void* b_scales, long l
 // 17568 x 2304 x 768 32.0 / 30.2 / 34.7 us, 24000 x 5120 x 768 (246 MB) - / 88.7 / 93.5, 33360 x 4096 x 768 (273 MB)
 // 124 / 109 / 93, 33360 x 4096 x 1536 - / 202 / 147.
 constexpr int kMxKeep = 16, kMxStream = 2;
+constexpr int kMxRingSteps = 24;  // mx_ring_kernel takes at least 4
 
 template <int MI>
 void mx_skinny_launch(const MxArgs& g, hipStream_t s) {
@@ -772,7 +757,7 @@ void mx_product(const MxArgs& g, hipStream_t st) {
   // 256 x 128: 4096^3 38.5 : 44.1 us, 8448 x 1280 x 5120 40.4 : 48.6, 33360 x 4096 x 3840 316 : 353, 8192^3 294 : 335; but
   // 16384 x 1280 x 5120 (1.25 rounds) 82.8 : 76.8, 16384 x 2560 x 2560 74.5 : 68.7, 33360 x 4096 x 768 116 : 93.
   const long rounds = (tiles2 + 255) / 256;
-  if (g.steps >= 24 && tiles2 > 128 && rounds * 102 < tiles2 * 127 / 256 + 20) {
+  if (g.steps >= kMxRingSteps && tiles2 > 128 && rounds * 102 < tiles2 * 127 / 256 + 20) {
     const dim3 grid((unsigned)tiles2);
     if (!vec) hipLaunchKernelGGL((mx_ring_kernel<false, 0>), grid, dim3(512), mx_ring_lds(), st, g);
     else if (stream) hipLaunchKernelGGL((mx_ring_kernel<true, kMxStream>), grid, dim3(512), mx_ring_lds(), st, g);
@@ -877,7 +862,7 @@ extern "C" int vpt_mxfp4_dequantize(const void* codes, long ldc, const void* sca
 extern "C" int vpt_gemm_mxfp4(const void* a_codes, long lda, const void* a_scales, long ldas, const void* b_codes,
                               long ldb, const void* b_scales, long ldbs, void* C, long ldc, int M, int N, int K,
                               const void* bias, const void* resid, long ldr, int f32_out, void* stream) {
-  VPT_CHECK_ARG(M >= 0 && N > 0 && K > 0 && K <= (1 << 30), "vpt_gemm_mxfp4: M >= 0, N > 0, 0 < K <= 2^30");
+  VPT_CHECK_ARG(M >= 0 && M <= (1 << 30) && N > 0 && N <= (1 << 30) && K > 0 && K <= (1 << 30), "vpt_gemm_mxfp4: 0 <= M, 0 < N, K <= 2^30");
   if (M == 0) return VPT_OK;
   const int steps = (K + 127) / 128;
   VPT_CHECK_ARG(a_codes && a_scales, "vpt_gemm_mxfp4: null pointer");
@@ -903,7 +888,7 @@ extern "C" int vpt_linear_mxfp4(const void* x, int dtype, long ldx, const void* 
                                 long ldws, void* y, long ldy, int M, int N, int K, const void* bias, const void* resid, long ldr,
                                 int f32_out, void* workspace, void* stream) {
   VPT_CHECK_ARG(dtype >= MX_BF16 && dtype <= MX_F16, "vpt_linear_mxfp4: dtype 0 bf16, 1 f32, 2 f16");
-  VPT_CHECK_ARG(M >= 0 && N > 0 && K > 0 && K <= (1 << 30), "vpt_linear_mxfp4: M >= 0, N > 0, 0 < K <= 2^30");
+  VPT_CHECK_ARG(M >= 0 && M <= (1 << 30) && N > 0 && N <= (1 << 30) && K > 0 && K <= (1 << 30), "vpt_linear_mxfp4: 0 <= M, 0 < N, K <= 2^30");
   if (M == 0) return VPT_OK;
   const int es = dtype == MX_F32 ? 4 : 2;
   VPT_CHECK_ARG(x && aligned(x, es) && (ldx >= K || M == 1), "vpt_linear_mxfp4: x aligned to its type, ldx >= K");

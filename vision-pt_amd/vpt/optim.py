@@ -228,8 +228,8 @@ class GradClip:
             if not want_norm:
                 ops.call("vpt_grad_list_clip", table, count, self._in_place, None, 0, 0.0, clip_value, None, st)
                 return None
-            ws = torch.empty(self._parts + 1, dtype=torch.float64, device=self.device)
-            norm = ws[self._parts:].view(torch.float32)[0]
+            ws = torch.empty(self._parts, dtype=torch.float64, device=self.device)
+            norm = torch.empty((), dtype=torch.float32, device=self.device)
             ops.call("vpt_grad_list_norm", table, self._count, ws.data_ptr(), st)
             ops.call("vpt_grad_list_clip", table, count, self._in_place, ws.data_ptr(), self._parts, max_norm, clip_value,
                      norm.data_ptr(), st)
