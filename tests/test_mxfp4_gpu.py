@@ -261,7 +261,9 @@ def test_no_rows(m):
     assert ops.mxfp4_dequantize(*ops.mxfp4_quantize(x), 40).shape == (0, 40)
 
 
-@pytest.mark.parametrize("M,N,K", [(1, 8, 8), (1, 64, 136), (5, 128, 256), (130, 264, 520), (300, 1280, 640)])
+@pytest.mark.parametrize("M,N,K", [(1, 8, 8), (1, 64, 136), (5, 128, 256), (130, 264, 520), (300, 1280, 640), (1, 2304, 768),
+                                   (16, 2304, 768), (3, 4096, 264), (64, 5120, 136), (129, 1032, 1000), (700, 2304, 768),
+                                   (3000, 2304, 768), (40, 136, 5120)])
 def test_dgrad(m, M, N, K):
     """dx = dy . W against 64 bits, bf16 inputs (the bound of the module's head with N additions)."""
     ops, mxfp4 = m
@@ -274,6 +276,12 @@ def test_dgrad(m, M, N, K):
     wide = torch.zeros(M + 1, N + 8, dtype=BF16, device=DEV)
     wide[:M, 8:].copy_(dy)
     assert torch.equal(ops.linear_mxfp4_dgrad(wide[:M, 8:], w).double(), dx)
+    assert torch.equal(ops.linear_mxfp4_dgrad(dy, w, out=torch.empty(M, K, dtype=BF16, device=DEV)).double(), dx)
+    buf = torch.full((M + 2, K + 16), 3.0, dtype=BF16, device=DEV)
+    into = ops.linear_mxfp4_dgrad(dy, w, out=buf[1:M + 1, 8:K + 8]).double()
+    assert ((into - ref).abs() <= (N + 3) * 2.0 ** -23 * top + 2.0 ** -8 * ref.abs()).all()
+    buf[1:M + 1, 8:K + 8] = 3.0
+    assert (buf == 3.0).all()
 
 
 def test_dgrad_against_differences(m):

@@ -1450,6 +1450,20 @@ def linear_mxfp4(x, w, bias=None, resid=None, out=None, out_dtype=BF16):
     return out
 
 
+def _mx_dgrad_splits(M: int, N: int, K: int) -> int:
+    """Slices of the reduction over N for dx [M, K] of few rows: its 128 x 128 tiles leave CUs idle, and each takes 0.9 us
+    per 64 of N; a slice's partial sums (f32) are written and read at about 5 TB/s and cost 3.5 us of launch. Measured
+    with W's dequantisation, one slice : the slices chosen (N x K, M): 2304 x 768, 1 38.0 : 15.0 us, 512 41.0 : 25.6,
+    4224 43.6 : 39.6; 5120 x 1280, 1 79.1 : 24.0, 1000 81.7 : 42.9, 2000 82.0 : 61.0; 1280 x 5120, 1 29.9 : 20.0, 256
+    37.4 : 28.5; with two slices where one is chosen, the product alone: 1280 x 5120, 512 24.9 : 25.3, 1000 29.0 : 41.5."""
+    tiles = -(-M // 128) * -(-K // 128)
+    cost = {1: 0.9 * N / 64}
+    for s in (2, 4, 8, 16):
+        if N // s >= 64 and tiles * s <= 512:
+            cost[s] = 0.9 * N / 64 / s + 3.5 + s * M * K * 8 / 5e6
+    return min(cost, key=cost.get)
+
+
 def linear_mxfp4_dgrad(dy, w, out=None):
     """dx = dy . W: the input gradient of linear_mxfp4, straight through the rounding of its input (dy [M, N] bf16, dx
     [M, K] bf16). W is dequantised to bf16 (exact) and goes through the bf16 GEMM, whose rows start at multiples of 16
@@ -1472,8 +1486,10 @@ def linear_mxfp4_dgrad(dy, w, out=None):
     if M == 0:
         return out
     dense = lambda t: t if M > 1 else t.as_strided(t.shape, (t.shape[1], 1))  # noqa: E731 (one row: any stride)
+    splits = _mx_dgrad_splits(M, N, K) if M == 1 or out.stride(0) == K else 1  # the slices' sum needs a dense out
+    tile = dict(splits=splits, geometry=128) if splits > 1 else {}
     with _on(dev):  # linear_dgrad launches on the current device
-        linear_dgrad(dense(dy), mxfp4_dequantize(w.codes, w.scales, K), out=dense(out))
+        linear_dgrad(dense(dy), mxfp4_dequantize(w.codes, w.scales, K), out=dense(out), **tile)
     return out
 
 
