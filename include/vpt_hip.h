@@ -221,7 +221,7 @@ int vpt_qknorm_rope_bwd_rows(const void* dqk, long lddqk, const void* qkv, long 
 int vpt_reduce_rows(const float* in, int R, int C, float* out, int accumulate, void* stream);
 
 /* ---- the end of a gated block and the next norm, fused --------------------------------------
- * M = groups * rows tokens of D values (D % 8 == 0, D <= 10240), group g = rows [g * rows, (g + 1) * rows):
+ * M = groups * rows <= 2^30 tokens of D values (D % 8 == 0, D <= 10240), groups < 2^24; group g = rows [g * rows, (g + 1) * rows):
  *   x_out = x + resid_scale * gate * (h * rsqrt(mean h^2 + eps) * w_post)   (w_post null: h itself; gate null: 1)
  *   y = x_out * rsqrt(mean x_out^2 + eps) * w_pre * (1 + scale) + shift      (w_pre null: no y; scale, shift null: 1, 0)
  * y is the norm of x_out as stored. h, y bf16; x, x_out bf16, or f32 with x_f32; vectors bf16 [D] (ld 0) or one row per

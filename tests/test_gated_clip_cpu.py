@@ -133,3 +133,20 @@ def test_c_abi_refuses_clip(m):
         a = list(ok)
         a[i] = v
         assert lib.vpt_grad_list_clip(*a) == 1, (i, v)
+
+
+def test_limits(m):
+    """Sizes beyond what a launch covers, limits that f32 holds as zero."""
+    ops, optim, _lib = m
+    p, lib = 4096, _lib.lib  # never read
+    fwd = [p, 16, p, 0, 16, p, p, p, 16, p, 16, p, 0, p, 16, p, 16, p, p, 3, 2, 16, 1.0, 1e-6, None]
+    bwd = [p, 16, p, 16, p, 16, p, 0, 16, p, p, p, p, p, 16, p, 16, p, 0, p, 16, p, 16, p, p, p, p, p, p, 3, 2, 16, 1.0, None]
+    for groups, rows in [(1 << 24, 1), (1, (1 << 30) + 1), (1 << 23, 129)]:
+        fwd[19:21], bwd[29:31] = (groups, rows), (groups, rows)
+        assert lib.vpt_gated_norm_fwd(*fwd) == 1 and lib.vpt_gated_norm_bwd(*bwd) == 1
+    handle = optim.GradClip.__new__(optim.GradClip)
+    for kw in (dict(max_norm=1e-50), dict(clip_value=1e-50), dict(max_norm=float("nan")), dict(clip_value=0.0), dict(max_norm=-1.0)):
+        with pytest.raises(ValueError, match="must be > 0"):
+            handle.clip(**kw)
+    with pytest.raises(ValueError, match="max_norm"):
+        optim.clip_grad_norm_([], 1e-50)

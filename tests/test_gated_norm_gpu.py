@@ -315,3 +315,29 @@ def test_far_offsets(ops):
     a = ops.gated_norm_bwd(dy, dxn, h, want[0], want[2], want[3], **kw)
     b = ops.gated_norm_bwd(v[4].copy_(dy), v[5].copy_(dxn), v[0], v[2], got[2], got[3], dh=v[1], dx=v[3], **kw)
     assert all(torch.equal(s, t) for s, t in zip(a, b))
+
+
+def test_more_rows_than_blocks(ops):
+    """2^28 + 40 rows of 8 columns, 16 to a block: more than one round of them per block; sampled rows against 64 bits, the
+    whole by a second half that repeats the first."""
+    half_rows, D = (1 << 27) + 20, 8
+    h = torch.empty(2, half_rows, D, dtype=BF16, device=DEV)
+    x = torch.empty_like(h)
+    g = torch.Generator(DEV).manual_seed(3)
+    for t in (h, x):
+        t[0].normal_(generator=g)
+        t[1].copy_(t[0])
+    w = 1 + rnd(D, seed=4, scale=0.2)
+    x_new, y, rh, rx = ops.gated_norm_fwd(h.view(-1, D), x.view(-1, D), w_post=w, w_pre=w, eps=EPS, x_out=x.view(-1, D))
+    for t in (x_new, y, rh, rx):
+        a, b = t.view(2, -1)
+        assert torch.equal(a, b)
+    at = torch.randint(half_rows, (4096,), device=DEV, generator=g)
+    u = h[0, at].double()
+    r = torch.rsqrt(u.square().mean(1, keepdim=True) + EPS)
+    ok(rh[:half_rows][at], r[:, 0], E1 * r[:, 0], "rstd_post")
+    xs = x_new.view(2, half_rows, D)[0, at].double()
+    r = torch.rsqrt(xs.square().mean(1, keepdim=True) + EPS)
+    ok(rx[:half_rows][at], r[:, 0], E1 * r[:, 0], "rstd_pre")
+    ref = xs * r * w.double()
+    ok(y.view(2, half_rows, D)[0, at], ref, 2.0 ** -8 * ref.abs() * 1.01 + E1 * ref.abs(), "y")

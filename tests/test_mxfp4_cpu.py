@@ -137,3 +137,23 @@ def test_c_abi_refuses(m):
     assert lib.vpt_mxfp4_quantize(None, 0, 256, 0, 256, None, 128, None, 8, None) == 0
     assert lib.vpt_mxfp4_dequantize(None, 128, None, 8, 0, 256, None, 256, 0, None) == 0
     assert lib.vpt_gemm_mxfp4(None, 128, None, 8, None, 128, None, 8, None, 64, 0, 64, 256, None, None, 0, 0, None) == 0
+
+
+def test_limits(m):
+    """Sizes beyond what a launch covers: more rows than an int holds, and more tiles than a grid."""
+    ops, lib = m[0], m[2].lib
+    many = torch.zeros(1, 64, dtype=torch.bfloat16, device="meta").expand((1 << 32) + 4, 64)
+    for t in (many, torch.empty((1 << 31), 1, dtype=torch.bfloat16, device="meta")):
+        with pytest.raises(ValueError, match=r"2\^31"):
+            ops.mxfp4_quantize(t)
+    p = 4096  # never read
+    for M, N in [(64, (1 << 27) + 1), (1 << 30, 257), (1 << 20, 1 << 20)]:
+        assert lib.vpt_gemm_mxfp4(p, 64, p, 4, p, 64, p, 4, p, N, M, N, 64, None, None, 0, 0, None) == 1
+        assert lib.vpt_linear_mxfp4(p, 0, 64, p, 64, p, 4, p, N, M, N, 64, None, None, 0, 0, p, None) == 1
+
+
+def test_out_is_not_x(m):
+    x = torch.zeros(2, 64, dtype=torch.bfloat16)
+    w = type("W", (), dict(shape=(64, 64), codes=torch.zeros(64, 64, dtype=torch.uint8), scales=torch.zeros(64, 4, dtype=torch.uint8)))
+    with pytest.raises(ValueError, match="out is x"):
+        m[0].linear_mxfp4(x, w, out=x)

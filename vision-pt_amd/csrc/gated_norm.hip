@@ -531,7 +531,8 @@ extern "C" long vpt_gated_norm_bwd_workspace(int groups, int rows, int D) {
 }
 
 #define VPT_GN_SHAPE(name)                                                                                             \
-  VPT_CHECK_ARG(groups >= 0 && rows >= 0 && (long)groups * rows < (1L << 31), name ": groups, rows >= 0, groups * rows < 2^31"); \
+  VPT_CHECK_ARG(groups >= 0 && rows >= 0 && groups < (1 << 24) && (long)groups * rows <= (1L << 30),                   \
+                name ": 0 <= groups < 2^24, 0 <= rows, groups * rows <= 2^30");                                         \
   VPT_CHECK_ARG(D > 0 && D % 8 == 0 && D <= kGnMaxD, name ": D a multiple of 8, at most 10240");                       \
   VPT_CHECK_ARG(!scale == !shift, name ": scale and shift go together");                                               \
   VPT_CHECK_ARG(w_pre || !scale, name ": a modulation needs w_pre")
@@ -564,6 +565,7 @@ extern "C" int vpt_gated_norm_fwd(const void* h, long ldh, const void* x, int x_
   g.rstd_post = rstd_post; g.rstd_pre = rstd_pre;
   g.rows = rows; g.D = D;
   g.rpb = 256 / gn_tpr(D);
+  while ((long)groups * ((rows + g.rpb - 1) / g.rpb) >= 1L << 24) g.rpb *= 2;  // a grid has under 2^32 threads
   g.bpg = (rows + g.rpb - 1) / g.rpb;
   g.s = resid_scale; g.eps = eps;
   gn_fwd_dispatch(g, groups * g.bpg, x_f32 != 0, (hipStream_t)stream);
@@ -596,7 +598,6 @@ extern "C" int vpt_gated_norm_bwd(const void* dy, long lddy, const void* dx_new,
   z.groups = groups; z.D = D;
   z.gate_each = ldg != 0; z.scale_each = lds != 0; z.shift_each = ldsh != 0;
   z.s = resid_scale;
-  VPT_CHECK_ARG((long)groups * gn_blocks_per_group(groups, rows > 0 ? rows : 1, D) < (1L << 31), "vpt_gated_norm_bwd: too many groups");
   VPT_CHECK_ARG(M > 0 || !sums, "vpt_gated_norm_bwd: no rows to sum over");
   if (M == 0) return VPT_OK;
   VPT_CHECK_ARG(h && dh && (!w_post || rstd_post) && (!w_pre || (dy && x_new && rstd_pre && dx)) && (w_pre || dx_new),

@@ -714,7 +714,7 @@ int mx_check_product(const void* b_codes, long ldb, const void* b_scales, long l
   VPT_CHECK_ARG((ldc >= N || M == 1) && aligned(C, f32_out ? 4 : 2), "mxfp4 product: output rows of N values, aligned to their type");
   VPT_CHECK_ARG((!bias || aligned(bias, 2)) && (!resid || (aligned(resid, 2) && (ldr >= N || M == 1))),
                 "mxfp4 product: bf16 bias and residual, rows of N values");
-  VPT_CHECK_ARG(((M + 127L) / 128) * ((N + 127L) / 128) < (1L << 31), "mxfp4 product: too many tiles");
+  VPT_CHECK_ARG(((M + 127L) / 128) * ((N + 127L) / 128) < (1L << 24), "mxfp4 product: too many tiles");  // a grid has under 2^32 threads
   return VPT_OK;
 }
 
@@ -862,7 +862,7 @@ extern "C" int vpt_mxfp4_dequantize(const void* codes, long ldc, const void* sca
 extern "C" int vpt_gemm_mxfp4(const void* a_codes, long lda, const void* a_scales, long ldas, const void* b_codes,
                               long ldb, const void* b_scales, long ldbs, void* C, long ldc, int M, int N, int K,
                               const void* bias, const void* resid, long ldr, int f32_out, void* stream) {
-  VPT_CHECK_ARG(M >= 0 && M <= (1 << 30) && N > 0 && N <= (1 << 30) && K > 0 && K <= (1 << 30), "vpt_gemm_mxfp4: 0 <= M, 0 < N, K <= 2^30");
+  VPT_CHECK_ARG(M >= 0 && M <= (1 << 30) && N > 0 && N <= (1 << 27) && K > 0 && K <= (1 << 30), "vpt_gemm_mxfp4: 0 <= M <= 2^30, 0 < N <= 2^27, 0 < K <= 2^30");
   if (M == 0) return VPT_OK;
   const int steps = (K + 127) / 128;
   VPT_CHECK_ARG(a_codes && a_scales, "vpt_gemm_mxfp4: null pointer");
@@ -888,7 +888,7 @@ extern "C" int vpt_linear_mxfp4(const void* x, int dtype, long ldx, const void* 
                                 long ldws, void* y, long ldy, int M, int N, int K, const void* bias, const void* resid, long ldr,
                                 int f32_out, void* workspace, void* stream) {
   VPT_CHECK_ARG(dtype >= MX_BF16 && dtype <= MX_F16, "vpt_linear_mxfp4: dtype 0 bf16, 1 f32, 2 f16");
-  VPT_CHECK_ARG(M >= 0 && M <= (1 << 30) && N > 0 && N <= (1 << 30) && K > 0 && K <= (1 << 30), "vpt_linear_mxfp4: 0 <= M, 0 < N, K <= 2^30");
+  VPT_CHECK_ARG(M >= 0 && M <= (1 << 30) && N > 0 && N <= (1 << 27) && K > 0 && K <= (1 << 30), "vpt_linear_mxfp4: 0 <= M <= 2^30, 0 < N <= 2^27, 0 < K <= 2^30");
   if (M == 0) return VPT_OK;
   const int es = dtype == MX_F32 ? 4 : 2;
   VPT_CHECK_ARG(x && aligned(x, es) && (ldx >= K || M == 1), "vpt_linear_mxfp4: x aligned to its type, ldx >= K");

@@ -1311,11 +1311,13 @@ def _rows2d(t, fn: str, arg: str, dtypes, shape=None, align: int = 1):
     bytes."""
     sh = t.shape
     if (t.dtype in dtypes and (len(sh) == 2 if shape is None else sh == shape) and t.is_contiguous()
-            and (align == 1 or not (t.data_ptr() % align or sh[0] > 1 and sh[1] * t.element_size() % align))):
+            and (align == 1 or not (t.data_ptr() % align or sh[0] > 1 and sh[1] * t.element_size() % align))
+            and sh[0] < 1 << 31 and sh[1] < 1 << 31):
         return
     _need(t.dtype in dtypes, f"{fn}: {arg}: dtype {t.dtype}, expected one of {[str(d) for d in dtypes]}")
     _need(t.dim() == 2 and (shape is None or tuple(t.shape) == tuple(shape)),
           f"{fn}: {arg}: shape {tuple(t.shape)}, expected {'[rows, cols]' if shape is None else tuple(shape)}")
+    _need(max(t.shape) < 1 << 31, f"{fn}: {arg}: shape {tuple(t.shape)}: fewer than 2^31 rows and columns")
     _need(t.shape[1] <= 1 or t.stride(1) == 1, f"{fn}: {arg}: the last dim must be contiguous")
     _need(t.shape[0] <= 1 or t.stride(0) >= t.shape[1], f"{fn}: {arg}: rows must not overlap (row stride {t.stride(0)})")
     _need(t.data_ptr() % align == 0 and (t.shape[0] <= 1 or t.stride(0) * t.element_size() % align == 0),
@@ -1432,12 +1434,14 @@ def gemm_mxfp4(a_codes, a_scales, w, out=None, *, bias=None, resid=None, out_dty
 def linear_mxfp4(x, w, bias=None, resid=None, out=None, out_dtype=BF16):
     """y = q(x) . W^T (+ bias) (+ resid): nn.Linear on an MXFP4 weight with its input quantised to MXFP4 on the way
     (x [M, K] bf16, f16 or f32; w a vpt.mxfp4.MXFP4Weight [N, K]): mxfp4_quantize and gemm_mxfp4, in one launch for a few rows.
-    y is bf16 or f32; `out` may be `resid` itself."""
+    y is bf16 or f32; `out` may be `resid` itself, but not share memory with x."""
     _rows2d(x, "linear_mxfp4", "x", _MX_DTYPES)
     M, K = x.shape
     N = w.shape[0]
     if K != w.shape[1]:
         raise ValueError(f"linear_mxfp4: x {tuple(x.shape)} does not match W {w.shape}")
+    if out is not None and out.data_ptr() == x.data_ptr() and M:
+        raise ValueError("linear_mxfp4: out is x")
     out = _mx_out("linear_mxfp4", M, N, x.device, bias, resid, out, out_dtype)
     dev = _gpu("linear_mxfp4", x, w.codes, w.scales, out, bias, resid)
     if M == 0:

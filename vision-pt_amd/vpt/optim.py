@@ -135,6 +135,7 @@ class RAdamScheduleFreeFlat:
 
 # ----------------------------------------------------------------------------- clipping of many gradient tensors
 _CLIP_DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
+_TINY = 2.0 ** -149  # the smallest f32 above 0, which would switch a limit off
 _PIECE = np.dtype([("g", "<u8"), ("out", "<u8"), ("n", "<i4"), ("dtype", "<i4")])  # VptGradPiece
 
 
@@ -240,10 +241,10 @@ class GradClip:
         """out = clamp(min(1, max_norm / (norm + 1e-6)) * g, -clip_value, clip_value); returns the norm before it (f32, on the
         device, not synchronised; None without max_norm). A gradient that is not finite makes the norm, and with it the
         clipped gradients, what torch.nn.utils.clip_grad_norm_ makes of them."""
-        if max_norm is not None and not max_norm > 0:
-            raise ValueError("max_norm must be > 0")
-        if clip_value is not None and not clip_value > 0:
-            raise ValueError("clip_value must be > 0")
+        if max_norm is not None and not max_norm >= _TINY:
+            raise ValueError("max_norm must be > 0 (as f32)")
+        if clip_value is not None and not clip_value >= _TINY:
+            raise ValueError("clip_value must be > 0 (as f32)")
         if max_norm is None and clip_value is None:
             raise ValueError("clip: max_norm or clip_value")
         return self._run(float(max_norm or 0.0), float(clip_value or 0.0), self._count, max_norm is not None)
@@ -261,8 +262,8 @@ def clip_grad_norm_(parameters, max_norm: float, clip_value: float | None = None
     params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     grads = [p.grad for p in params if p.grad is not None]
     if not grads:
-        if not max_norm > 0:
-            raise ValueError("max_norm must be > 0")
+        if not max_norm >= _TINY:
+            raise ValueError("max_norm must be > 0 (as f32)")
         return torch.tensor(0.0)
     clipper = GradClip(grads)
     if error_if_nonfinite and not bool(torch.isfinite(clipper.norm())):
