@@ -150,3 +150,31 @@ def test_limits(m):
             handle.clip(**kw)
     with pytest.raises(ValueError, match="max_norm"):
         optim.clip_grad_norm_([], 1e-50)
+
+
+def test_clip_grad_norm_has_torchs_positions(m, monkeypatch):
+    """The third positional argument is torch's norm_type (L2 alone is offered), never the value limit."""
+    optim = m[1]
+    calls = []
+
+    class Handle:
+        def __init__(self, grads, out=None):
+            pass
+
+        def norm(self):
+            return torch.tensor(1.0)
+
+        def clip(self, max_norm=None, clip_value=None):
+            calls.append((max_norm, clip_value))
+            return torch.tensor(1.0)
+    monkeypatch.setattr(optim, "GradClip", Handle)
+    p = torch.nn.Parameter(z(3, d=F32))
+    p.grad = z(3, d=F32)
+    optim.clip_grad_norm_([p], 10.0, 2.0)
+    optim.clip_grad_norm_([p], 10.0, 2, True)
+    optim.clip_grad_norm_([p], 10.0, error_if_nonfinite=True, clip_value=0.5)
+    assert calls == [(10.0, None), (10.0, None), (10.0, 0.5)]
+    for kind in (float("inf"), 1.0, 0.02, float("nan")):
+        for grads in ([p], []):
+            with pytest.raises(ValueError, match="norm_type"):
+                optim.clip_grad_norm_(grads, 1.0, kind)

@@ -255,10 +255,13 @@ class GradClip:
         return self._run(0.0, 0.0, 0, True)
 
 
-def clip_grad_norm_(parameters, max_norm: float, clip_value: float | None = None,
-                    error_if_nonfinite: bool = False) -> torch.Tensor:
-    """torch.nn.utils.clip_grad_norm_ (L2) over parameters' .grad, then clip_grad_value_ when clip_value is given, in place.
-    Parameters without a gradient are left out; error_if_nonfinite reads the norm back before anything is scaled."""
+def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False, *,
+                    clip_value: float | None = None) -> torch.Tensor:
+    """torch.nn.utils.clip_grad_norm_ over parameters' .grad (its positions; norm_type 2 alone), then clip_grad_value_ when
+    clip_value is given, in place. Parameters without a gradient are left out; error_if_nonfinite reads the norm back before
+    anything is scaled."""
+    if float(norm_type) != 2.0:
+        raise ValueError(f"clip_grad_norm_: norm_type {norm_type}: the L2 norm (2.0) is the only one")
     params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     grads = [p.grad for p in params if p.grad is not None]
     if not grads:
