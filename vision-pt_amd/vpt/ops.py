@@ -11,6 +11,7 @@ import contextlib
 import ctypes
 from typing import NamedTuple
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -1331,6 +1332,47 @@ def _vec1d(t, fn: str, arg: str, dtype, n: int, align: int = 1):
         raise ValueError(f"{fn}: {arg} at a multiple of {align} bytes")
 
 
+def _bytes2d(t) -> tuple[int, int, int, int]:
+    """(first byte, rows, bytes between rows, bytes of a row) of a checked [rows, cols] or contiguous tensor."""
+    es = t.element_size()
+    if t.dim() == 2:
+        return t.data_ptr(), t.shape[0], t.stride(0) * es, t.shape[1] * es
+    return t.data_ptr(), 1, 0, t.numel() * es
+
+
+def _share(a, b) -> bool:
+    """Whether two checked tensors (rows contiguous, not overlapping) have a byte in common."""
+    a0, ra, sa, la = _bytes2d(a)
+    b0, rb, sb, lb = _bytes2d(b)
+    if not (ra and rb and la and lb) or a0 + (ra - 1) * sa + la <= b0 or b0 + (rb - 1) * sb + lb <= a0:
+        return False
+    if ra > 1 and rb > 1 and sa == sb:  # columns of one wider tensor: row j of b lies d bytes behind row j + q of a
+        q, d = divmod(b0 - a0, sa)
+        met = lambda q: max(0, -q) < min(rb, ra - q)  # noqa: E731 (a row j of b with a row j + q of a)
+        return d < la and met(q) or d + lb > sa and met(q + 1)
+    if ra > rb:
+        a0, ra, sa, la, b0, rb, sb, lb = b0, rb, sb, lb, a0, ra, sa, la
+    if rb == 1:
+        return True
+    for lo in range(0, ra, 1 << 20):  # per row of a: the rows of b that begin before its end and end behind its begin
+        at = np.arange(lo, min(ra, lo + (1 << 20)), dtype=np.int64) * sa + (a0 - b0)
+        if (np.maximum((at - lb) // sb + 1, 0) <= np.minimum((at + la - 1) // sb, rb - 1)).any():
+            return True
+    return False
+
+
+def _apart(fn: str, arg: str, out, others, same=()):
+    """`out`, which a call writes, shares no memory with what it reads: [(name, tensor or None)] of `others`, nor of `same`
+    unless it is that tensor itself (the same rows of the same type: each value is read before it is written)."""
+    for name, t in same:
+        if t is not None and not (t.data_ptr() == out.data_ptr() and t.dtype == out.dtype and t.shape == out.shape
+                                  and _ld(t) == _ld(out)) and _share(out, t):
+            raise ValueError(f"{fn}: {arg} shares memory with {name}")
+    for name, t in others:
+        if t is not None and _share(out, t):
+            raise ValueError(f"{fn}: {arg} shares memory with {name}")
+
+
 def _ld(t) -> int:
     """The row stride of a checked [rows, cols] tensor; a single row has the stride of a dense one."""
     return t.stride(0) if t.shape[0] > 1 else max(1, t.shape[1])
@@ -1375,6 +1417,9 @@ def mxfp4_quantize(x, codes=None, scales=None):
         scales = torch.empty(ss, dtype=torch.uint8, device=x.device)
     if given:
         _mx_parts(codes, scales, M, K, "mxfp4_quantize")
+        _apart("mxfp4_quantize", "codes", codes, (("x", x),))
+        _apart("mxfp4_quantize", "scales", scales, (("x", x),))
+        _need(not _share(codes, scales), "mxfp4_quantize: codes and scales share memory")
     dev = _gpu("mxfp4_quantize", x, codes, scales)
     if M == 0:
         return codes, scales
@@ -1393,6 +1438,7 @@ def mxfp4_dequantize(codes, scales, K: int, out=None, dtype=BF16):
         out = torch.empty(M, K, dtype=dtype, device=codes.device)
     else:
         _rows2d(out, "mxfp4_dequantize", "out", _MX_OUT, (M, K))
+        _apart("mxfp4_dequantize", "out", out, (("codes", codes), ("scales", scales)))
     dev = _gpu("mxfp4_dequantize", codes, scales, out)
     if M == 0:
         return out
@@ -1401,27 +1447,31 @@ def mxfp4_dequantize(codes, scales, K: int, out=None, dtype=BF16):
     return out
 
 
-def _mx_out(fn, M, N, dev, bias, resid, out, out_dtype):
-    if out is None:
+def _mx_out(fn, M, N, dev, w, reads, bias, resid, out, out_dtype):
+    """The result of a product that reads `reads` [(name, tensor)]: checked, or allocated."""
+    given = out is not None
+    if given:
+        _rows2d(out, fn, "out", _MX_OUT, (M, N))
+    else:
         _need(out_dtype in _MX_OUT, f"{fn}: out bf16 or f32")
         out = torch.empty(M, N, dtype=out_dtype, device=dev)
-    else:
-        _rows2d(out, fn, "out", _MX_OUT, (M, N))
     if bias is not None:
         _vec1d(bias, fn, "bias", BF16, N)
     if resid is not None:
         _rows2d(resid, fn, "resid", (BF16,), (M, N))
+    if given:
+        _apart(fn, "out", out, (*reads, ("W's codes", w.codes), ("W's scales", w.scales), ("bias", bias)), (("resid", resid),))
     return out
 
 
 def gemm_mxfp4(a_codes, a_scales, w, out=None, *, bias=None, resid=None, out_dtype=BF16):
     """out[M, N] = A . W^T (+ bias) (+ resid) of two MXFP4 matrices on the scaled matrix instruction: A as mxfp4_quantize
     gives it, w a vpt.mxfp4.MXFP4Weight [N, K]. f32 accumulation, bias and residual added in f32, one rounding to out's type
-    (bf16 or f32). `out` may be `resid` itself. See csrc/mxfp4.hip."""
+    (bf16 or f32). `out` may be `resid` itself, and shares memory with no other operand. See csrc/mxfp4.hip."""
     N, K = w.shape
     M = a_codes.shape[0]
     _mx_parts(a_codes, a_scales, M, K, "gemm_mxfp4")
-    out = _mx_out("gemm_mxfp4", M, N, a_codes.device, bias, resid, out, out_dtype)
+    out = _mx_out("gemm_mxfp4", M, N, a_codes.device, w, (("a_codes", a_codes), ("a_scales", a_scales)), bias, resid, out, out_dtype)
     dev = _gpu("gemm_mxfp4", a_codes, a_scales, w.codes, w.scales, out, bias, resid)
     if M == 0:
         return out
@@ -1434,7 +1484,7 @@ def gemm_mxfp4(a_codes, a_scales, w, out=None, *, bias=None, resid=None, out_dty
 def linear_mxfp4(x, w, bias=None, resid=None, out=None, out_dtype=BF16):
     """y = q(x) . W^T (+ bias) (+ resid): nn.Linear on an MXFP4 weight with its input quantised to MXFP4 on the way
     (x [M, K] bf16, f16 or f32; w a vpt.mxfp4.MXFP4Weight [N, K]): mxfp4_quantize and gemm_mxfp4, in one launch for a few rows.
-    y is bf16 or f32; `out` may be `resid` itself, but not share memory with x."""
+    y is bf16 or f32; `out` may be `resid` itself, and shares memory with no other operand (blocks read x after others wrote)."""
     _rows2d(x, "linear_mxfp4", "x", _MX_DTYPES)
     M, K = x.shape
     N = w.shape[0]
@@ -1442,7 +1492,7 @@ def linear_mxfp4(x, w, bias=None, resid=None, out=None, out_dtype=BF16):
         raise ValueError(f"linear_mxfp4: x {tuple(x.shape)} does not match W {w.shape}")
     if out is not None and out.data_ptr() == x.data_ptr() and M:
         raise ValueError("linear_mxfp4: out is x")
-    out = _mx_out("linear_mxfp4", M, N, x.device, bias, resid, out, out_dtype)
+    out = _mx_out("linear_mxfp4", M, N, x.device, w, (("x", x),), bias, resid, out, out_dtype)
     dev = _gpu("linear_mxfp4", x, w.codes, w.scales, out, bias, resid)
     if M == 0:
         return out
@@ -1486,6 +1536,7 @@ def linear_mxfp4_dgrad(dy, w, out=None):
         out = torch.empty(M, K, dtype=BF16, device=dy.device)
     else:
         _rows2d(out, "linear_mxfp4_dgrad", "out", (BF16,), (M, K), 16)
+        _apart("linear_mxfp4_dgrad", "out", out, (("dy", dy), ("W's codes", w.codes), ("W's scales", w.scales)))
     dev = _gpu("linear_mxfp4_dgrad", dy, w.codes, w.scales, out)
     if M == 0:
         return out
@@ -1539,6 +1590,15 @@ def _gn_vec(v):
     return (None, 0) if v is None else (v.data_ptr(), 0 if v.dim() == 1 else _ld(v))
 
 
+def _gn_apart(fn, a, b, rows, vecs):
+    """The given results a, b (name, tensor or None) may each be one of the row operands, and share no other memory."""
+    for n, t in (a, b):
+        if t is not None:
+            _apart(fn, n, t, vecs, rows)
+    if a[1] is not None and b[1] is not None:
+        _need(not _share(a[1], b[1]), f"{fn}: {a[0]} and {b[0]} share memory")
+
+
 def gated_norm_fwd(h, x, *, w_post=None, w_pre=None, gate=None, scale=None, shift=None, groups: int = 1,
                    resid_scale: float = 1.0, eps: float = 1e-6, x_out=None, y=None):
     """The end of a gated block and the next block's norm in one pass (vpt_gated_norm_fwd):
@@ -1549,13 +1609,15 @@ def gated_norm_fwd(h, x, *, w_post=None, w_pre=None, gate=None, scale=None, shif
     h [M, D] bf16 the block's output, x [M, D] the residual stream (bf16 or f32; x_new has its type and may be x: `x_out`).
     Each vector may be left out: w_post (h enters as it is), gate, w_pre (no y), scale and shift. gate, scale and shift are
     [D], or [groups, D] with one row for each of `groups` equal runs of rows (a sample's tokens); rows of a wider tensor do.
-    y is the norm of x_new as it is stored. D % 8 == 0, D <= 10240, rows at multiples of 16 bytes.
+    y is the norm of x_new as it is stored. D % 8 == 0, D <= 10240, rows at multiples of 16 bytes. `x_out` and `y` may each be
+    x or h itself, and share no other memory with what is read or with each other.
     Returns (x_new, y, rstd_post, rstd_pre), the last two f32 [M] for gated_norm_bwd; None where there is no such norm."""
     _rows2d(h, "gated_norm_fwd", "h", _BF16)
     M, D = h.shape
     _gn_params("gated_norm_fwd", D, M, groups, w_post, w_pre, gate, scale, shift)
     _rows2d(h, "gated_norm_fwd", "h", _BF16, (M, D), 16)
     _rows2d(x, "gated_norm_fwd", "x", _MX_OUT, (M, D), 16)
+    given = ("x_out", x_out), ("y", y)
     if x_out is None:
         x_out = torch.empty(M, D, dtype=x.dtype, device=x.device)
     else:
@@ -1565,6 +1627,8 @@ def gated_norm_fwd(h, x, *, w_post=None, w_pre=None, gate=None, scale=None, shif
         _rows2d(y, "gated_norm_fwd", "y", _BF16, (M, D), 16)
     elif w_pre is not None:
         y = torch.empty(M, D, dtype=BF16, device=x.device)
+    _gn_apart("gated_norm_fwd", *given, (("h", h), ("x", x)),
+              (("w_post", w_post), ("w_pre", w_pre), ("gate", gate), ("scale", scale), ("shift", shift)))
     dev = _gpu("gated_norm_fwd", h, x, w_post, w_pre, gate, scale, shift, x_out, y)
     rstd_post = None if w_post is None else torch.empty(M, dtype=F32, device=x.device)
     rstd_pre = None if w_pre is None else torch.empty(M, dtype=F32, device=x.device)
@@ -1580,9 +1644,11 @@ def gated_norm_bwd(dy, dx_new, h, x_new, rstd_post, rstd_pre, *, w_post=None, w_
                    shift=None, groups: int = 1, resid_scale: float = 1.0, dh=None, dx=None) -> GatedNormGrads:
     """The gradients of gated_norm_fwd, from dy (of y; None without w_pre) and dx_new (of x_new from what follows; None: zero,
     only with w_pre), with h, x_new and the rstd of the forward and its vectors. The vectors' gradients are sums over rows
-    in a fixed order (the same bits every time). Without w_pre dx is dx_new itself, nothing is copied. dh may be h, and dx
-    dx_new (each element is read before it is written)."""
+    in a fixed order (the same bits every time). Without w_pre dx is dx_new itself, nothing is copied. dh and dx may each be
+    dy, dx_new, h or x_new itself (each element is read before it is written), and share no other memory with what is read
+    or with each other."""
     fn = "gated_norm_bwd"
+    given = ("dh", dh), ("dx", dx)
     _rows2d(h, fn, "h", _BF16)
     M, D = h.shape
     _gn_params(fn, D, M, groups, w_post, w_pre, gate, scale, shift)
@@ -1605,6 +1671,7 @@ def gated_norm_bwd(dy, dx_new, h, x_new, rstd_post, rstd_pre, *, w_post=None, w_
         _need(dx is None, "gated_norm_bwd: without w_pre dx is dx_new")
         _rows2d(dx_new, fn, "dx_new", _MX_OUT, (M, D), 16)
         dx, kind, x_new, rstd_pre = dx_new, dx_new.dtype, None, None
+        _need(dh is None or not _share(dh, dx), "gated_norm_bwd: dh and dx_new share memory (without w_pre dx is dx_new)")
     if w_post is not None:
         _need(rstd_post is not None, "gated_norm_bwd: rstd_post missing")
         _vec1d(rstd_post, fn, "rstd_post", F32, M)
@@ -1614,6 +1681,9 @@ def gated_norm_bwd(dy, dx_new, h, x_new, rstd_post, rstd_pre, *, w_post=None, w_
         dh = torch.empty(M, D, dtype=BF16, device=h.device)
     else:
         _rows2d(dh, fn, "dh", _BF16, (M, D), 16)
+    _gn_apart(fn, *given, (("dy", dy), ("dx_new", dx_new), ("h", h), ("x_new", x_new)),
+              (("rstd_post", rstd_post), ("rstd_pre", rstd_pre), ("w_post", w_post), ("w_pre", w_pre), ("gate", gate),
+               ("scale", scale), ("shift", shift)))
     dev = _gpu("gated_norm_bwd", h, dy, dx_new, x_new, rstd_post, rstd_pre, w_post, w_pre, gate, scale, shift, dh, dx)
     vecs = (w_post, w_pre, gate, scale, shift)
     make = torch.empty if M else torch.zeros
