@@ -191,3 +191,74 @@ def test_sdxl_block_on_mxfp4(m):
         res.append([y, dx, dctx] + [t.clone() for lin in blk.lin.values() for t in (lin.g_up, lin.g_down)])
     assert all(torch.isfinite(t.float()).all() and t.float().abs().max() > 0 for t in res[0])
     assert all(torch.equal(p, q) for p, q in zip(*res))
+
+
+@pytest.mark.parametrize("mode", ["dequant"])
+def test_lora_on_two_streams(m, mode):
+    """Two LoRA targets of one size over different MXFP4 bases, forward and backward under way on two streams at once: each
+    gives what it gives alone (the dequantised bases, split-K slabs and adapter-gradient slabs are a stream's own)."""
+    from vpt.sdxl import LoRALinearNF4
+    ops, mx, _ = m
+    N, K, M = 1280, 5120, 500  # the forward splits its reduction
+    lins, ins = [], []
+    for k in (0, 1):
+        w = mx.MXFP4Weight.quantize(rnd(N, K, seed=10 + k, scale=K ** -0.5))
+        lins.append(LoRALinearNF4(w, rnd(N, seed=20 + k), rnd(16, K, seed=30 + k, scale=0.05), rnd(N, 16, seed=40 + k, scale=0.05),
+                                  alpha=16.0, rank=16, base_mode=mode))
+        ins.append((rnd(M, K, seed=50 + k), rnd(M, N, seed=60 + k)))
+
+    def step(lin, x, dy):
+        lin.g_up.zero_()
+        lin.g_down.zero_()
+        return lin.forward(x), lin.backward(dy), lin.g_up, lin.g_down
+    want = [[t.clone() for t in step(lin, *i)] for lin, i in zip(lins, ins)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for lin in lins:
+        lin.base.resident = None  # the first use is on the side stream, the next on another
+    torch.cuda.synchronize()
+    for _ in range(4):
+        got = []
+        for lin, i, s in zip(lins, ins, streams):
+            with torch.cuda.stream(s):
+                for _ in range(3):
+                    out = step(lin, *i)
+                got.append(out)
+        streams.reverse()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_lora_captured_twice(m):
+    """Two graphs of two LoRA targets share no scratch, and an eager call that needs a larger one takes none from them."""
+    from vpt.sdxl import LoRALinearNF4
+    ops, mx, _ = m
+    lins, ins, want, graphs, res = [], [], [], [], []
+    for k, (N, K) in enumerate([(1280, 5120), (1280, 5120), (2560, 5120)]):
+        w = mx.MXFP4Weight.quantize(rnd(N, K, seed=10 + k, scale=K ** -0.5))
+        lins.append(LoRALinearNF4(w, None, rnd(16, K, seed=30 + k, scale=0.05), rnd(N, 16, seed=40 + k, scale=0.05), alpha=16.0,
+                                  rank=16, base_mode="dequant"))
+        ins.append((rnd(400, K, seed=50 + k), rnd(400, N, seed=60 + k)))
+
+    def step(lin, x, dy):
+        lin.g_up.zero_()
+        lin.g_down.zero_()
+        return lin.forward(x), lin.backward(dy), lin.g_up, lin.g_down
+    for lin, i in zip(lins[:2], ins):
+        want.append([t.clone() for t in step(lin, *i)])
+    for lin, i in zip(lins[:2], ins):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            res.append(step(lin, *i))
+        graphs.append(g)
+    side = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(3):
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, side):
+            with torch.cuda.stream(s):
+                g.replay()
+        step(lins[2], *ins[2])
+        torch.cuda.synchronize()
+        for a, b in zip(res, want):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
+        step(lins[0], *ins[0])

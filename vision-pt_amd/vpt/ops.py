@@ -132,29 +132,47 @@ def gemm(a, a_kmajor: bool, b, b_kmajor: bool, M: int, N: int, K: int, out, *, b
     return out
 
 
-_WS: dict = {}  # (device, tag) -> f32 workspace grown on demand (stream-ordered reuse on one stream)
+def _here(dev) -> tuple[int, int]:
+    """The index of a GPU and its current stream: what a scratch buffer belongs to."""
+    index = torch.device(dev).index
+    if index is None:
+        index = torch.cuda.current_device()
+    return index, torch._C._cuda_getCurrentRawStream(index)
+
+
+def _capturing() -> bool:
+    return torch.cuda.is_current_stream_capturing()
+
+
+def _scratch(cache: dict, dev, tag, n: int, dtype, make=torch.empty) -> torch.Tensor:
+    """A buffer of at least n elements for launches on the current stream of dev, grown on demand. One per (device, stream,
+    tag): the launches of a stream run in order, those of two streams do not. In a captured region it is a new one from the
+    graph's memory each time, so that graphs replayed at once share none and none goes back to the allocator when an eager
+    call lets its buffer grow; the caller holds it until the launches that use it are recorded."""
+    if _capturing():
+        return make(n, dtype=dtype, device=dev)
+    key = (*_here(dev), tag)
+    buf = cache.get(key)
+    if buf is None or buf.numel() < n or buf.dtype != dtype:
+        buf = cache[key] = make(n, dtype=dtype, device=dev)
+    return buf
+
+
+_WS: dict = {}  # (device, stream, tag) -> workspace
 
 
 def workspace(dev, tag: str, n: int, dtype=F32) -> torch.Tensor:
-    """A per-(device, tag) buffer of at least n elements, grown on demand (stream-ordered reuse)."""
-    buf = _WS.get((str(dev), tag))
-    if buf is None or buf.numel() < n or buf.dtype != dtype:
-        buf = _WS[(str(dev), tag)] = torch.empty(n, dtype=dtype, device=dev)
-    return buf[:n]
+    """n elements of scratch for the launches of the current stream (_scratch)."""
+    return _scratch(_WS, dev, tag, n, dtype)[:n]
 
 
-_TICKETS: dict = {}  # (device, stream) -> zero-filled u32 tickets of the in-launch row-block reductions
+_TICKETS: dict = {}  # (device, stream, "") -> zero-filled u32 tickets of the in-launch row-block reductions
 
 
 def tickets(dev, n: int) -> torch.Tensor:
     """Row-block tickets for a kernel whose in-launch reduction counts blocks on them (vpt_geglu_bwd_lora /
-    vpt_geglu_fwd_lora): zero when allocated, left zero by every launch, so one buffer serves every shape; one per
-    (device, current stream), so launches on one stream reuse it in order and two streams never share tickets."""
-    key = (str(dev), stream())
-    buf = _TICKETS.get(key)
-    if buf is None or buf.numel() < n:
-        buf = _TICKETS[key] = torch.zeros(max(n, 1024), dtype=torch.int32, device=dev)
-    return buf
+    vpt_geglu_fwd_lora): zero when allocated, left zero by every launch, so one buffer serves every shape of a stream."""
+    return _scratch(_TICKETS, dev, "", max(n, 1024), torch.int32, torch.zeros)
 
 
 GEO_R2_128 = 1281  # 128 x 128 tiles on the R2 ring's pipeline (include/vpt_hip.h vpt_gemm_bf16_tiled)
@@ -1107,14 +1125,11 @@ def lora_proj(x, w, w_kmajor: bool, out, alpha=1.0):
     return out
 
 
-_LORA_WS: dict = {}  # per (device, tag, bytes): split slabs, reused across launches on one stream
+_LORA_WS: dict = {}  # per (device, stream, (tag, bytes)): split slabs, reused across launches on one stream
 
 
 def _lora_ws(dev, tag, nbytes):
-    ws = _LORA_WS.get((dev, tag, nbytes))
-    if ws is None:
-        ws = _LORA_WS[(dev, tag, nbytes)] = torch.empty(nbytes // 4, dtype=F32, device=dev)
-    return ws
+    return _scratch(_LORA_WS, dev, (tag, nbytes), nbytes // 4, F32)
 
 
 class _LoraReduceJob(ctypes.Structure):
@@ -1138,7 +1153,7 @@ class _LoraBatch:
     def __init__(self, side=None):
         self.jobs: list = []
         self.pjobs: list = []  # deferred slab jobs
-        self.keep: list = []   # their operand tensors
+        self.keep: list = []   # their operand tensors, and the slabs until the reduce
         self.key = None  # (alpha, accumulate) of the pending jobs
         self.nws = 0     # workspaces handed out since the last flush
         self.side = side  # a stream the flushes run on (beside the caller's), or None
@@ -1152,7 +1167,9 @@ class _LoraBatch:
 
     def ws(self, dev, nbytes):
         self.nws += 1
-        return _lora_ws(dev, f"batch{self.nws}", nbytes)
+        ws = _lora_ws(dev, f"batch{self.nws}", nbytes)
+        self.keep.append(ws)
+        return ws
 
     def add(self, jobs):
         assert len(self.jobs) + len(jobs) <= 32

@@ -97,7 +97,7 @@ class NF4Weight:
 #   "dequant"  (default) bitsandbytes' MatMul4Bit semantics (bnb 0.48.2 matmul_4bit for a multi-row input:
 #              dequantize_4bit(W) to a bf16 weight, then F.linear; its backward dequantises again): each forward and
 #              each input-gradient call dequantises W (vpt_nf4_dequant, 16-B vectorised, HBM-bound) into one
-#              per-device scratch and runs the bf16 ring / T128 GEMM with the LoRA term as a K-extension
+#              scratch of the stream and runs the bf16 ring / T128 GEMM with the LoRA term as a K-extension
 #              (vpt_gemm_bf16_lora). Only the NF4 state stays resident.
 #   "resident" the dequantised bf16 base kept in HBM next to its NF4 state (frozen, so it is computed once; 4.4 GB
 #              for the SDXL UNet's transformer Linears -- room the 288 GB of an MI355X has), same GEMMs.
@@ -106,14 +106,10 @@ class NF4Weight:
 # All three give the same dequantised values; "dequant" and "resident" give bitwise identical outputs.
 BASE_MODES = ("dequant", "resident", "inline")
 DEFAULT_BASE_MODE = "dequant"
-_SCRATCH: dict = {}  # (device, "call" | "block") -> bf16 dequant scratch, grown on demand
 
 
 def _dequant_scratch(base: "NF4Weight", device) -> torch.Tensor:
-    buf = _SCRATCH.get((str(device), "call"))
-    if buf is None or buf.numel() < base.numel:
-        buf = _SCRATCH[(str(device), "call")] = torch.empty(base.numel, dtype=BF16, device=device)
-    return base.dequantize(buf[:base.numel].view(base.shape))
+    return base.dequantize(ops.workspace(device, "base_call", base.numel, BF16).view(base.shape))
 
 
 def dequant_into(pairs):
@@ -126,7 +122,7 @@ def dequant_into(pairs):
 
 def dequant_bases(lins: dict, targets, device) -> dict:
     """{target: bf16 base} for a block's LoRA targets about to run: "dequant" mode dequantises all of them in ONE
-    launch (vpt_nf4_dequant_batch) into a shared per-device scratch (stream-ordered reuse, block after block);
+    launch (vpt_nf4_dequant_batch) into the stream's scratch (reused block after block, ops.workspace);
     "resident" returns the kept bf16 bases; "inline" (or a non-fused target) returns nothing (the GEMM dequantises)."""
     ts = [t for t in targets if lins[t].fused and lins[t].base_mode != "inline"]
     if not ts:
@@ -140,9 +136,7 @@ def dequant_bases(lins: dict, targets, device) -> dict:
             out["attn1.qkv"] = q.resident_qkv
         return out
     total = sum(lins[t].base.numel for t in ts)
-    buf = _SCRATCH.get((str(device), "block"))
-    if buf is None or buf.numel() < total:
-        buf = _SCRATCH[(str(device), "block")] = torch.empty(total, dtype=BF16, device=device)
+    buf = ops.workspace(device, "base_block", total, BF16)
     out, off = {}, 0
     for t in ts:
         b = lins[t].base
