@@ -193,7 +193,7 @@ def test_sdxl_block_on_mxfp4(m):
     assert all(torch.equal(p, q) for p, q in zip(*res))
 
 
-@pytest.mark.parametrize("mode", ["dequant"])
+@pytest.mark.parametrize("mode", ["dequant", "resident"])
 def test_lora_on_two_streams(m, mode):
     """Two LoRA targets of one size over different MXFP4 bases, forward and backward under way on two streams at once: each
     gives what it gives alone (the dequantised bases, split-K slabs and adapter-gradient slabs are a stream's own)."""

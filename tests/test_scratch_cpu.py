@@ -84,3 +84,57 @@ def test_batched_slabs_are_held(at):
     b = ops._LoraBatch()
     ptrs = [b.ws(torch.device("cpu"), 4096).data_ptr() for _ in range(4)]
     assert len(set(ptrs)) == 4 and {t.data_ptr() for t in b.keep} >= set(ptrs)
+
+
+class Event:
+    made = []
+
+    def __init__(self):
+        self.recorded = None
+        Event.made.append(self)
+
+    def record(self, stream=None):
+        self.recorded = stream
+
+
+class Stream:
+    def __init__(self, name):
+        self.name, self.waits = name, []
+
+    def wait_event(self, e):
+        self.waits.append(e)
+
+
+class Kept(torch.Tensor):
+    """A tensor that notes the streams it is marked as used on."""
+    def record_stream(self, s):
+        self.__dict__.setdefault("used", []).append(s.name)
+
+
+@pytest.mark.parametrize("attr", ["resident", "resident_qkv", "anything"])
+def test_built_once_is_waited_for(at, monkeypatch, attr):
+    """A base kept on the device is built on the stream of its first caller; another stream waits for that, once, and its use is
+    known to the allocator; a capture keeps nothing whose values only a replay would make."""
+    ops, _, state = at
+    streams = {k: Stream(k) for k in (11, 12, 13)}
+    monkeypatch.setattr(torch.cuda, "Event", Event)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda dev=None: streams[state["stream"]])
+    owner, builds = type("Owner", (), dict(resident=None, resident_qkv=None))(), []
+
+    def build():
+        builds.append(state["stream"])
+        return torch.zeros(4).as_subclass(Kept)
+    state["capturing"] = True
+    t = ops.built_once(owner, attr, build)
+    assert getattr(owner, attr, None) is None and builds == [11]
+    state["capturing"] = False
+    t = ops.built_once(owner, attr, build)
+    assert builds == [11, 11] and getattr(owner, attr) is t and ops.built_once(owner, attr, build) is t
+    assert not streams[11].waits and Event.made[-1].recorded is streams[11]
+    for s in (12, 13, 12, 11):
+        state["stream"] = s
+        assert ops.built_once(owner, attr, build) is t
+    assert [len(streams[s].waits) for s in (11, 12, 13)] == [0, 1, 1] and t.used == [12, 13] and builds == [11, 11]
+    state["stream"], state["capturing"] = 14, True  # an event from outside may not enter a capture
+    streams[14] = Stream(14)
+    assert ops.built_once(owner, attr, build) is t and not streams[14].waits

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import weakref
 from typing import NamedTuple
 
 import numpy as np
@@ -164,6 +165,33 @@ _WS: dict = {}  # (device, stream, tag) -> workspace
 def workspace(dev, tag: str, n: int, dtype=F32) -> torch.Tensor:
     """n elements of scratch for the launches of the current stream (_scratch)."""
     return _scratch(_WS, dev, tag, n, dtype)[:n]
+
+
+_BUILT = weakref.WeakKeyDictionary()  # owner -> {attr: (tensor, event behind its launches, streams it is ready on)}
+
+
+def built_once(owner, attr: str, build) -> torch.Tensor:
+    """owner.attr, a device tensor that `build` makes on its first use and that is kept. Its launches are on the first caller's
+    stream: a caller on another one waits for them (once per stream). In a captured region what is not there yet is made for
+    the graph alone (its values exist only once the graph has run); what is there was made before, and torch.cuda.graph
+    synchronises before it begins."""
+    t = getattr(owner, attr, None)
+    if _capturing():
+        return build() if t is None else t
+    if t is None:
+        t = build()
+        done = torch.cuda.Event()
+        done.record(torch.cuda.current_stream(t.device))
+        setattr(owner, attr, t)
+        _BUILT.setdefault(owner, {})[attr] = (t, done, {_here(t.device)})
+        return t
+    made, done, seen = _BUILT.get(owner, {}).get(attr, (None, None, ()))
+    if made is t and _here(t.device) not in seen:
+        st = torch.cuda.current_stream(t.device)
+        st.wait_event(done)
+        t.record_stream(st)
+        seen.add(_here(t.device))
+    return t
 
 
 _TICKETS: dict = {}  # (device, stream, "") -> zero-filled u32 tickets of the in-launch row-block reductions

@@ -130,10 +130,8 @@ def dequant_bases(lins: dict, targets, device) -> dict:
     if lins[ts[0]].base_mode == "resident":
         out = {t: base_weight(lins[t].base, "resident", device) for t in ts}
         if ts[:3] == QKV:
-            q = lins[QKV[0]].base
-            if q.resident_qkv is None:  # the stacked copy of the fused q|k|v GEMMs, kept with the q base
-                q.resident_qkv = torch.cat([out[t] for t in QKV], 0)
-            out["attn1.qkv"] = q.resident_qkv
+            # the stacked copy of the fused q|k|v GEMMs, kept with the q base
+            out["attn1.qkv"] = ops.built_once(lins[QKV[0]].base, "resident_qkv", lambda: torch.cat([out[t] for t in QKV], 0))
         return out
     total = sum(lins[t].base.numel for t in ts)
     buf = ops.workspace(device, "base_block", total, BF16)
@@ -152,9 +150,7 @@ def dequant_bases(lins: dict, targets, device) -> dict:
 def base_weight(base: "NF4Weight", mode: str, device) -> torch.Tensor:
     """The bf16 base weight a "dequant" / "resident" GEMM reads (stream-ordered scratch reuse for "dequant")."""
     if mode == "resident":
-        if base.resident is None:
-            base.resident = base.dequantize()
-        return base.resident
+        return ops.built_once(base, "resident", base.dequantize)
     return _dequant_scratch(base, device)
 
 

@@ -190,10 +190,8 @@ class SDXLStacksQLoRA:
             G = len(group)
             ups = self.params[u0:u0 + G * w * r].view(G * w, r)
             if group[0].base_mode == "resident":
-                W = self._kv_resident.get(w) if hasattr(self, "_kv_resident") else None
-                if W is None:
-                    W = torch.cat([base_weight(l.base, "resident", self.device) for l in group], 0)
-                    self._kv_resident = {**getattr(self, "_kv_resident", {}), w: W}
+                W = ops.built_once(self, f"_kv_resident{w}", lambda: torch.cat(
+                    [base_weight(l.base, "resident", self.device) for l in group], 0))
             else:
                 W = ops.workspace(self.device, f"kv_base{w}", G * w * cd, BF16).view(G * w, cd)
                 dequant_into([(l.base, W[i * w:(i + 1) * w]) for i, l in enumerate(group)])
