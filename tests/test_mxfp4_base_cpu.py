@@ -1,0 +1,39 @@
+"""CPU: MXFP4 weights (and NF4 states of other classes) as frozen bases of the LoRA layers: where they are moved, which modes they
+take, which launch dequantises them."""
+
+import pytest
+import torch
+
+BF16, U8 = torch.bfloat16, torch.uint8
+
+
+@pytest.fixture(scope="module")
+def m():
+    from vpt import mxfp4, ops, sdxl
+    return ops, mxfp4, sdxl
+
+
+def weight(m, N, K):
+    c = -(-K // 128)
+    return m[1].MXFP4Weight(torch.zeros(N, 64 * c, dtype=U8), torch.zeros(N, 4 * c, dtype=U8), (N, K))
+
+
+def block_sd(m, dim=64, rank=16):
+    sd = {}
+    for t in m[2].TARGETS:
+        n, k = {"ff.net.0.proj": (8 * dim, dim), "ff.net.2": (dim, 4 * dim)}.get(t, (dim, dim))
+        sd[f"{t}.linear.weight"] = weight(m, n, k)
+        sd[f"{t}.lora_down.weight"], sd[f"{t}.lora_up.weight"] = torch.zeros(rank, k), torch.zeros(n, rank)
+    for k in ("norm1", "norm2", "norm3"):
+        sd[f"{k}.weight"], sd[f"{k}.bias"] = torch.ones(dim), torch.zeros(dim)
+    return sd
+
+
+def test_block_moves_its_bases(m):
+    """A state dict loaded elsewhere: bases follow the block's device as NF4 states, biases and adapters do."""
+    blk = m[2].SDXLTransformerBlock(64, 1, 64, 16, 16.0, block_sd(m), device="meta")
+    for t, lin in blk.lin.items():
+        assert lin.down.device.type == "meta" and lin.base.codes.device.type == "meta" and lin.base.scales.device.type == "meta", t
+    here = block_sd(m)
+    blk = m[2].SDXLTransformerBlock(64, 1, 64, 16, 16.0, here, device="cpu")
+    assert all(blk.lin[t].base is here[f"{t}.linear.weight"] for t in blk.lin)  # already there: the same weight, with what it keeps

@@ -62,4 +62,6 @@ class MXFP4Weight:
                                     None if out is None else out.view(self.shape), BF16)
 
     def to(self, device) -> "MXFP4Weight":
-        return MXFP4Weight(self.codes.to(device), self.scales.to(device), self.shape)
+        """On `device`: itself where it is there already."""
+        codes, scales = self.codes.to(device), self.scales.to(device)
+        return self if codes is self.codes and scales is self.scales else MXFP4Weight(codes, scales, self.shape)

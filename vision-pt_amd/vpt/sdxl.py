@@ -346,8 +346,7 @@ class SDXLTransformerBlock:
         self.lin = {}
         for t in TARGETS:
             base = sd[f"{t}.linear.weight"]
-            if not isinstance(base, MXFP4Weight):
-                base = _nf4_or_dense(base, code2, device)
+            base = base.to(device) if isinstance(base, MXFP4Weight) else _nf4_or_dense(base, code2, device)
             b = sd.get(f"{t}.linear.bias")
             self.lin[t] = LoRALinearNF4(base, None if b is None else b.to(device, BF16).contiguous(),
                                         sd[f"{t}.lora_down.weight"].to(device), sd[f"{t}.lora_up.weight"].to(device),
