@@ -37,3 +37,29 @@ def test_block_moves_its_bases(m):
     here = block_sd(m)
     blk = m[2].SDXLTransformerBlock(64, 1, 64, 16, 16.0, here, device="cpu")
     assert all(blk.lin[t].base is here[f"{t}.linear.weight"] for t in blk.lin)  # already there: the same weight, with what it keeps
+
+
+def lora(m, base, mode=None):
+    return m[2].LoRALinearNF4(base, None, torch.zeros(16, base.shape[1]), torch.zeros(base.shape[0], 16), 16.0, 16, mode)
+
+
+def test_base_mode_is_checked_when_set(m):
+    """The mode is assigned after construction too; "inline" reads NF4 parts, which an MXFP4 base has not."""
+    lin = lora(m, weight(m, 64, 64))
+    assert lin.base_mode == "dequant"
+    lin.base_mode = "resident"
+    for mode, what in [("inline", "inline"), ("fast", "base_mode"), (None, "base_mode")]:
+        with pytest.raises(ValueError, match=what):
+            lin.base_mode = mode
+        assert lin.base_mode == "resident"
+    with pytest.raises(ValueError, match="inline"):
+        lora(m, weight(m, 64, 64), "inline")
+    nf4 = m[2].NF4Weight(*[torch.zeros(1)] * 5, (64, 64))
+    lin = lora(m, nf4)
+    lin.base_mode = "inline"
+    proj = m[2].NF4Linear(nf4, None, "inline")
+    assert lin.base_mode == proj.base_mode == "inline"
+    with pytest.raises(ValueError, match="base_mode"):
+        proj.base_mode = "fast"
+    with pytest.raises(ValueError, match="inline"):
+        m[2].NF4Linear(weight(m, 64, 64), None, "inline")

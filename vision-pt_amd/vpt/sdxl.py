@@ -154,7 +154,23 @@ def base_weight(base: "NF4Weight", mode: str, device) -> torch.Tensor:
     return _dequant_scratch(base, device)
 
 
-class LoRALinearNF4:
+class _BaseMode:
+    """The `base_mode` of a layer over a frozen `base`: checked when it is set, also after construction."""
+
+    @property
+    def base_mode(self) -> str:
+        return self._base_mode
+
+    @base_mode.setter
+    def base_mode(self, mode: str):
+        if mode not in BASE_MODES:
+            raise ValueError(f"base_mode must be one of {BASE_MODES}")
+        if mode == "inline" and isinstance(self.base, MXFP4Weight):
+            raise ValueError("base_mode \"inline\" dequantises NF4 inside the GEMM: an NF4Weight only")
+        self._base_mode = mode
+
+
+class LoRALinearNF4(_BaseMode):
     """a29. `down` [r, in], `up` [out, r] bf16 trainable (grads `g_down`, `g_up` f32); `base` NF4 [out, in] (an NF4Weight), or
     a vpt.mxfp4.MXFP4Weight in the "dequant" and "resident" modes (its bf16 values take the place of NF4's).
 
@@ -170,10 +186,6 @@ class LoRALinearNF4:
                  alpha: float, rank: int, base_mode: str | None = None):
         self.base, self.bias = base, bias
         self.base_mode = base_mode or DEFAULT_BASE_MODE
-        if self.base_mode not in BASE_MODES:
-            raise ValueError(f"base_mode must be one of {BASE_MODES}")
-        if self.base_mode == "inline" and not isinstance(base, NF4Weight):
-            raise ValueError("base_mode \"inline\" dequantises NF4 inside the GEMM: an NF4Weight only")
         self.down, self.up = down.to(BF16).contiguous(), up.to(BF16).contiguous()
         self.scale = alpha / rank
         self.g_down = torch.zeros(self.down.shape, dtype=F32, device=self.down.device)
@@ -589,7 +601,7 @@ class SDXLTransformerBlock:
         return out
 
 
-class NF4Linear:
+class NF4Linear(_BaseMode):
     """A frozen NF4 Linear without adapters (SpatialTransformer proj_in / proj_out): vpt_gemm_nf4 both ways."""
 
     def __init__(self, base: NF4Weight, bias: torch.Tensor | None, base_mode: str | None = None):
