@@ -63,3 +63,20 @@ def test_base_mode_is_checked_when_set(m):
         proj.base_mode = "fast"
     with pytest.raises(ValueError, match="inline"):
         m[2].NF4Linear(weight(m, 64, 64), None, "inline")
+
+
+def test_every_base_is_dequantised(m, monkeypatch):
+    """dequant_into: MXFP4 bases by their own launch, every other one (NF4 states of any class) in the batched launches."""
+    ops, _, sdxl = m
+    batched, own = [], []
+    monkeypatch.setattr(ops, "nf4_dequant_batch", lambda pairs: batched.append([b for b, _ in pairs]))
+
+    class Like:  # the parts of an NF4Weight, of a class of its own
+        pass
+    mx = weight(m, 64, 64)
+    mx.dequantize = lambda out=None: own.append(out)
+    nf4, like, out = m[2].NF4Weight(*[torch.zeros(1)] * 5, (64, 64)), Like(), torch.zeros(1)
+    sdxl.dequant_into([(nf4, None), (mx, out), (like, None)])
+    assert batched == [[nf4, like]] and own == [out]
+    like.shape, like.numel = (64, 64), 4096
+    assert lora(m, like, "inline").base is like

@@ -114,7 +114,7 @@ def _dequant_scratch(base: "NF4Weight", device) -> torch.Tensor:
 
 def dequant_into(pairs):
     """[(base, bf16 out)]: the NF4 bases in one launch per 16 (vpt_nf4_dequant_batch), MXFP4 bases one by one."""
-    ops.nf4_dequant_batch([(b, o) for b, o in pairs if isinstance(b, NF4Weight)])
+    ops.nf4_dequant_batch([(b, o) for b, o in pairs if not isinstance(b, MXFP4Weight)])
     for b, o in pairs:
         if isinstance(b, MXFP4Weight):
             b.dequantize(o)
