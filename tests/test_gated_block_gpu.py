@@ -262,3 +262,20 @@ def test_lora_captured_twice(m):
         for a, b in zip(res, want):
             assert all(torch.equal(p, q) for p, q in zip(a, b))
         step(lins[0], *ins[0])
+
+
+def test_frozen_linear_on_mxfp4(m):
+    """A frozen Linear without adapters over an MXFP4 base, both ways against 64 bits: f32 sums and one rounding to bf16."""
+    from vpt.sdxl import NF4Linear
+    ops, mx, _ = m
+    N, K = 320, 640
+    w, bias = mx.MXFP4Weight.quantize(rnd(N, K, seed=1, scale=K ** -0.5)), rnd(N, seed=2)
+    x, dy = rnd(150, K, seed=3), rnd(150, N, seed=4)
+    W = w.dequantize().double()
+    for mode in ("dequant", "resident"):
+        lin = NF4Linear(w, bias, mode)
+        for got, a, b, add in ((lin.forward(x), x, W.t(), bias), (lin.backward(dy), dy, W, None)):
+            ref, top = a.double() @ b, a.double().abs() @ b.abs()
+            if add is not None:
+                ref, top = ref + add.double(), top + add.double().abs()
+            assert ((got.double() - ref).abs() <= (a.shape[1] + 3) * 2.0 ** -23 * top + 2.0 ** -8 * ref.abs()).all()

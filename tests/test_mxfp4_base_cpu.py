@@ -80,3 +80,13 @@ def test_every_base_is_dequantised(m, monkeypatch):
     assert batched == [[nf4, like]] and own == [out]
     like.shape, like.numel = (64, 64), 4096
     assert lora(m, like, "inline").base is like
+
+
+def test_spatial_transformer_takes_them(m):
+    """proj_in and proj_out too, on the stack's device."""
+    sd = {f"transformer_blocks.0.{k}": v for k, v in block_sd(m).items()}
+    sd.update({"norm.weight": torch.ones(64), "norm.bias": torch.zeros(64), "proj_in.weight": weight(m, 64, 64),
+               "proj_in.bias": torch.zeros(64), "proj_out.weight": weight(m, 64, 64), "proj_out.bias": torch.zeros(64)})
+    st = m[2].SDXLSpatialTransformer(64, 1, 1, 64, 16, 16.0, sd, device="meta")
+    for p in (st.proj_in, st.proj_out):
+        assert isinstance(p.base, m[1].MXFP4Weight) and p.base.codes.device.type == "meta" and p.base_mode == "dequant"

@@ -357,8 +357,7 @@ class SDXLTransformerBlock:
         self.device = device
         self.lin = {}
         for t in TARGETS:
-            base = sd[f"{t}.linear.weight"]
-            base = base.to(device) if isinstance(base, MXFP4Weight) else _nf4_or_dense(base, code2, device)
+            base = _base(sd[f"{t}.linear.weight"], code2, device)
             b = sd.get(f"{t}.linear.bias")
             self.lin[t] = LoRALinearNF4(base, None if b is None else b.to(device, BF16).contiguous(),
                                         sd[f"{t}.lora_down.weight"].to(device), sd[f"{t}.lora_up.weight"].to(device),
@@ -602,7 +601,8 @@ class SDXLTransformerBlock:
 
 
 class NF4Linear(_BaseMode):
-    """A frozen NF4 Linear without adapters (SpatialTransformer proj_in / proj_out): vpt_gemm_nf4 both ways."""
+    """A frozen Linear without adapters (SpatialTransformer proj_in / proj_out) over an NF4 base (or an MXFP4Weight, not
+    "inline"): dequantised and a bf16 GEMM, or vpt_gemm_nf4 in "inline" mode, both ways."""
 
     def __init__(self, base: NF4Weight, bias: torch.Tensor | None, base_mode: str | None = None):
         self.base, self.bias = base, bias
@@ -623,7 +623,10 @@ class NF4Linear(_BaseMode):
         return ops.linear_dgrad(dy, base_weight(self.base, self.base_mode, dy.device), out=dx)
 
 
-def _nf4_or_dense(wt, code2, device):
+def _base(wt, code2, device):
+    """A frozen base from an MXFP4Weight, an NF4 state or a dense tensor (quantised to NF4), on the device."""
+    if isinstance(wt, MXFP4Weight):
+        return wt.to(device)
     if isinstance(wt, dict):
         return NF4Weight.from_state(wt, device)
     if code2 is None:
@@ -634,8 +637,8 @@ def _nf4_or_dense(wt, code2, device):
 class SDXLSpatialTransformer:
     """SpatialTransformer.forward (src/models/sdxl/denoiser.py:283-365) on the HIP kernels, QLoRA-trained:
     GroupNorm(32, C, eps 1e-6) on the NCHW stage activation (vpt_groupnorm_fwd) -> NCHW->tokens
-    (vpt_transpose_add) -> proj_in (NF4) -> `depth` SDXLTransformerBlocks (LoRA on their 10 Linears) ->
-    proj_out (NF4) -> tokens->NCHW + residual (vpt_transpose_add with the add fused). The backward returns the
+    (vpt_transpose_add) -> proj_in (NF4 or MXFP4) -> `depth` SDXLTransformerBlocks (LoRA on their 10 Linears) ->
+    proj_out (NF4 or MXFP4) -> tokens->NCHW + residual (vpt_transpose_add with the add fused). The backward returns the
     input and context gradients and accumulates every adapter's gradient (GroupNorm / proj weights frozen).
     State-dict names are the reference's (`norm.*`, `proj_in.*`, `transformer_blocks.{i}.<target>.linear.*`,
     `.lora_down.weight`, `.lora_up.weight`, `norm{1,2,3}.*`, `proj_out.*`)."""
@@ -647,9 +650,9 @@ class SDXLSpatialTransformer:
         self.device = device
         self.norm_w = sd["norm.weight"].to(device, BF16).contiguous()
         self.norm_b = sd["norm.bias"].to(device, BF16).contiguous()
-        self.proj_in = NF4Linear(_nf4_or_dense(sd["proj_in.weight"], code2, device),
+        self.proj_in = NF4Linear(_base(sd["proj_in.weight"], code2, device),
                                  sd["proj_in.bias"].to(device, BF16).contiguous())
-        self.proj_out = NF4Linear(_nf4_or_dense(sd["proj_out.weight"], code2, device),
+        self.proj_out = NF4Linear(_base(sd["proj_out.weight"], code2, device),
                                   sd["proj_out.bias"].to(device, BF16).contiguous())
         self.blocks = []
         for i in range(depth):
