@@ -279,3 +279,35 @@ def test_frozen_linear_on_mxfp4(m):
             if add is not None:
                 ref, top = ref + add.double(), top + add.double().abs()
             assert ((got.double() - ref).abs() <= (a.shape[1] + 3) * 2.0 ** -23 * top + 2.0 ** -8 * ref.abs()).all()
+
+
+def test_stacks_on_mxfp4(m):
+    """Transformer stacks of two widths whose every base is MXFP4: the stacked k / v projections against 64 bits (ds rounded to
+    bf16, 2^-8 of it, f32 sums, one rounding of the result), and a step's gradients, dequantised per block and kept."""
+    from vpt.sdxl_train import SDXLStacksQLoRA
+    ops, mx, _ = m
+    res = []
+    for mode in ("dequant", "resident"):
+        st = SDXLStacksQLoRA(B=2, stacks=[("a", 640, 10, 1, 16), ("b", 1280, 20, 2, 8)], n_ctx=77, seed=3)
+        g = torch.Generator(device=DEV).manual_seed(9)
+        st.params.copy_((torch.randn(st.params.shape, device=DEV, generator=g) * 0.03).bfloat16())
+        blocks = [blk for (_, _, _, s) in st.stacks for blk in s.blocks]
+        layers = [p for (_, _, _, s) in st.stacks for p in (s.proj_in, s.proj_out)] + [lin for b in blocks for lin in b.lin.values()]
+        for p in layers:
+            p.base = mx.MXFP4Weight.quantize(p.base.dequantize())
+            p.base_mode = mode
+        xs, ctx, gs = st.make_inputs(seed=4)
+        st.opt.step = lambda: None
+        res.append((st.step(xs, ctx, gs).clone(), st.grads.clone()))
+        assert st.precompute_ctx_kv(ctx)
+        X = ctx.double()
+        for blk in blocks:
+            for got, t in zip(blk.ctx_kv, ("attn2.to_k", "attn2.to_v")):
+                lin = blk.lin[t]
+                W, down, up = (v.double() for v in (lin.base.dequantize(), lin.down, lin.up))
+                ds = lin.scale * (X @ down.t())
+                ref = X @ W.t() + ds @ up.t()
+                tol = 2.0 ** -8 * (ref.abs() + ds.abs() @ up.abs().t()) * 1.01 + \
+                    (X.shape[1] + 32) * 2.0 ** -23 * (X.abs() @ W.abs().t() + lin.scale * (X.abs() @ down.abs().t()) @ up.abs().t())
+                assert ((got.double() - ref).abs() <= tol).all()
+    assert all(torch.equal(p, q) and torch.isfinite(p.float()).all() and p.float().abs().max() > 0 for p, q in zip(*res))
