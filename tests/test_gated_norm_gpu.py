@@ -341,3 +341,44 @@ def test_more_rows_than_blocks(ops):
     ok(rx[:half_rows][at], r[:, 0], E1 * r[:, 0], "rstd_pre")
     ref = xs * r * w.double()
     ok(y.view(2, half_rows, D)[0, at], ref, 2.0 ** -8 * ref.abs() * 1.01 + E1 * ref.abs(), "y")
+
+
+@pytest.mark.parametrize("D", [8, 72, 648, 1288, 2568, 10232])
+@pytest.mark.parametrize("name", ["w_post", "gate", "w_pre", "scale"])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("R", [5, 1])
+def test_not_finite_vectors(ops, D, name, bad, R):
+    """An infinity or a NaN in a vector's last value, at widths that leave lanes behind the row: forward and backward give what
+    the formula gives, finite where it is finite, a NaN where it is one, the same infinity elsewhere."""
+    G = 2
+    h, x, kw = make(G, R, D, F32, "pnGM", seed=5)
+    kw[name] = kw[name].clone()
+    kw[name][..., -1] = bad
+    vec = {k: rows(kw[k], G, R) for k in ("w_post", "w_pre", "gate", "scale", "shift")}
+
+    def same(got, ref, what):
+        assert torch.equal(got.isnan().cpu(), ref.isnan().cpu()), what
+        inf = ref.isinf()
+        assert torch.equal(got.double()[inf], ref[inf]) and torch.isfinite(got[torch.isfinite(ref)]).all(), what
+    u = h.double() * torch.rsqrt(h.double().square().mean(1, keepdim=True) + EPS) * vec["w_post"] * vec["gate"]
+    xn = x.double() + 0.7 * u
+    n = xn * torch.rsqrt(xn.square().mean(1, keepdim=True) + EPS)
+    x_new, y, rh, rx = ops.gated_norm_fwd(h, x, eps=EPS, **kw)
+    same(x_new, xn, "x_new")
+    same(y, n * vec["w_pre"] * (1 + vec["scale"]) + vec["shift"], "y")
+    # backward, at a finite stream
+    xf = x.double()
+    r, rr = torch.rsqrt(h.double().square().mean(1, keepdim=True) + EPS), torch.rsqrt(xf.square().mean(1, keepdim=True) + EPS)
+    dy, dxn = rnd(G * R, D, seed=50), rnd(G * R, D, dtype=F32, seed=51)
+    got = ops.gated_norm_bwd(dy, dxn, h, x, r[:, 0].float(), rr[:, 0].float(), **kw)
+    n, v = xf * rr, h.double() * r
+    dn = dy.double() * (1 + vec["scale"]) * vec["w_pre"]
+    dX = dxn.double() + rr * (dn - n * (dn * n).mean(1, keepdim=True))
+    dv = 0.7 * vec["gate"] * vec["w_post"] * dX
+    same(got.dx, dX, "dx")
+    same(got.dh, r * (dv - v * (dv * v).mean(1, keepdim=True)), "dh")
+    P, Q = ((t * u).view(G, R, D).sum(1) for t, u in ((dy.double(), n), (dX, v)))
+    wide = {k: kw[k].double() for k in ("w_post", "w_pre", "gate", "scale")}
+    for k, ref in (("dscale", wide["w_pre"] * P), ("dw_pre", ((1 + wide["scale"]) * P).sum(0)), ("dgate", 0.7 * wide["w_post"] * Q),
+                   ("dw_post", (0.7 * wide["gate"] * Q).sum(0)), ("dshift", dy.double().view(G, R, D).sum(1))):
+        same(getattr(got, k), ref, k)

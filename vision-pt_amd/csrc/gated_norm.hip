@@ -137,7 +137,7 @@ __global__ __launch_bounds__(256) void gated_norm_fwd_kernel(GnArgs g) {
     ss = 0.f;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int c = lane + TPR * i, cv = min(c, nch - 1);  // past the row: its last chunk's vectors, times zeros
+      const int c = lane + TPR * i, cv = min(c, nch - 1);  // past the row (in the last chunk): no value, no part in the mean
       float u[8], t[8];
       wh[i].get(u);
       wx[i].get(f[i]);
@@ -154,7 +154,7 @@ __global__ __launch_bounds__(256) void gated_norm_fwd_kernel(GnArgs g) {
         for (int e = 0; e < 8; ++e) u[e] *= t[e];
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[i][e] += u[e];
+      for (int e = 0; e < 8; ++e) f[i][e] = i == NC - 1 && c >= nch ? 0.f : f[i][e] + u[e];
       if (ok && c < nch) gn_store8<XF32>(g.xo, row * g.ldxo + c * 8, f[i]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss += f[i][e] * f[i][e];
@@ -252,7 +252,8 @@ __global__ __launch_bounds__(256, gn_bwd_occ(NC)) void gated_norm_bwd_kernel(GnA
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int c = min(lane + TPR * i, nch - 1);  // past the row: its last chunk's factors, times zeros
+      const int c = min(lane + TPR * i, nch - 1);
+      const bool on = ok && (i < NC - 1 || lane + TPR * i < nch);  // else no value: a factor may be infinite
       wd[i].get(dX[i]);
       if (g.w_pre) {
         float n[8], t[8];
@@ -267,7 +268,7 @@ __global__ __launch_bounds__(256, gn_bwd_occ(NC)) void gated_norm_bwd_kernel(GnA
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          dn[i][e] *= t[e];
+          dn[i][e] = on ? dn[i][e] * t[e] : 0.f;
           dot += dn[i][e] * n[e];
         }
       }
@@ -293,7 +294,7 @@ __global__ __launch_bounds__(256, gn_bwd_occ(NC)) void gated_norm_bwd_kernel(GnA
       for (int e = 0; e < 8; ++e) {
         v[e] *= rh;
         Q[i][e] += dX[i][e] * v[e];
-        dn[i][e] = dX[i][e] * t[e];  // from here on dn holds dv
+        dn[i][e] = i == NC - 1 && c >= nch ? 0.f : dX[i][e] * t[e];  // from here on dn holds dv
         dot += dn[i][e] * v[e];
       }
       if (g.xo && ok && c < nch) gn_store8<XF32>(g.xo, row * g.ldxo + c * 8, dX[i]);
