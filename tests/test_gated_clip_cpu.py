@@ -178,3 +178,23 @@ def test_clip_grad_norm_has_torchs_positions(m, monkeypatch):
         for grads in ([p], []):
             with pytest.raises(ValueError, match="norm_type"):
                 optim.clip_grad_norm_(grads, 1.0, kind)
+
+
+def handle(optim, grads, out=None):
+    """A GradClip without a GPU: its table on the CPU, no launch."""
+    c = optim.GradClip.__new__(optim.GradClip)
+    c.grads, c.out, c.device = grads, grads if out is None else out, torch.device("cpu")
+    return c
+
+
+def test_the_memory_of_the_table_stays(m, monkeypatch):
+    """The handle holds the memory that its table names, also when a tensor is given other memory meanwhile."""
+    ops, optim, _ = m
+    monkeypatch.setattr(ops, "_raw_stream", lambda index: 7)
+    monkeypatch.setattr(ops, "_capturing", lambda: False, raising=False)
+    g, o = z(40, d=F32), z(40, d=F32)
+    c = handle(optim, [g], [o])
+    c._finish()
+    mem = [t.untyped_storage().data_ptr() for t in (g, o)]
+    g.data, o.data = z(40, d=F32), z(40, d=F32)
+    assert {s.data_ptr() for s in c._memory} == set(mem)

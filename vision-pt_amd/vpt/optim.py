@@ -161,9 +161,10 @@ class GradClip:
 
     `grads`: dense GPU tensors of one device (bf16, f16 and f32 may be mixed; any dims, also transposed; empty ones too).
     `out`: tensors of the same types, shapes and strides for the clipped gradients; None: in place. What is written must not
-    overlap. The handle keeps the tensors and a table of them on the device: gradients that are new tensors every step
-    (`zero_grad(set_to_none=True)`) go through clip_grad_norm_ instead. Building it copies the table to the device and
-    is not for a captured region; clip() and norm() are (their workspace is allocated per call), and may run on any stream."""
+    overlap. The handle keeps the tensors, their memory as it was then, and a table of it on the device: gradients that are new
+    tensors every step (`zero_grad(set_to_none=True)`) go through clip_grad_norm_ instead, and a tensor that is given other
+    memory (`t.data = ...`, `set_`) needs a new handle. Building it copies the table to the device, waiting for that, and is
+    not for a captured region; clip() and norm() are (their workspace is allocated per call), and may run on any stream."""
 
     def __init__(self, grads, out=None):
         self.grads = list(grads)
@@ -198,8 +199,16 @@ class GradClip:
             raise ValueError("GradClip: tensors on different devices")
         self.device = devs.pop() if devs else torch.device("cuda", torch.cuda.current_device())
         with ops._on(self.device.index):
-            self._table, self._count = self._pieces()
-            self._stream = ops._raw_stream(self.device.index)
+            self._finish()
+
+    def _finish(self):
+        """The table of the checked tensors, and what it names: the memory stays this handle's, also when a tensor is given
+        other memory meanwhile (`t.data = ...`)."""
+        self._memory = [t.untyped_storage() for t in self.grads]
+        if self.out is not self.grads:
+            self._memory += [t.untyped_storage() for t in self.out]
+        self._table, self._count = self._pieces()
+        self._stream = ops._raw_stream(self.device.index)
         self._parts = ops.call("vpt_grad_list_parts", self._count)
         self._in_place = int(all(o.data_ptr() == g.data_ptr() for g, o in zip(self.grads, self.out)))
 
