@@ -187,6 +187,33 @@ def handle(optim, grads, out=None):
     return c
 
 
+def test_a_captured_table_stays(m, monkeypatch):
+    """A graph reads the handle's table at every replay, also when the handle is gone by then."""
+    import contextlib
+    import gc
+    import weakref
+    ops, optim, _ = m
+    state = {"capturing": False}
+    monkeypatch.setattr(ops, "_on", lambda index: contextlib.nullcontext())
+    monkeypatch.setattr(ops, "_raw_stream", lambda index: 7)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state["capturing"])
+    monkeypatch.setattr(ops, "_capturing", lambda: state["capturing"])
+    real = ops.call
+    monkeypatch.setattr(ops, "call", lambda name, *a: real(name, *a) if name.endswith(("_parts", "_piece")) else None)
+
+    def use(capturing):
+        c = handle(optim, [z(40, d=F32)])
+        c._finish()
+        state["capturing"] = capturing
+        c.clip(1.0)
+        c.clip(clip_value=1.0)
+        state["capturing"] = False
+        return weakref.ref(c._table)
+    tables = use(False), use(True)
+    gc.collect()
+    assert tables[0]() is None and tables[1]() is not None
+
+
 def test_the_memory_of_the_table_stays(m, monkeypatch):
     """The handle holds the memory that its table names, also when a tensor is given other memory meanwhile."""
     ops, optim, _ = m

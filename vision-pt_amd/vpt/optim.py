@@ -137,6 +137,7 @@ class RAdamScheduleFreeFlat:
 _CLIP_DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
 _TINY = 2.0 ** -149  # the smallest f32 above 0, which would switch a limit off
 _PIECE = np.dtype([("g", "<u8"), ("out", "<u8"), ("n", "<i4"), ("dtype", "<i4")])  # VptGradPiece
+_CAPTURED: list = []  # tables that captured graphs read at every replay: they stay when their handles go
 
 
 def _dense(t: torch.Tensor) -> bool:
@@ -164,7 +165,8 @@ class GradClip:
     overlap. The handle keeps the tensors, their memory as it was then, and a table of it on the device: gradients that are new
     tensors every step (`zero_grad(set_to_none=True)`) go through clip_grad_norm_ instead, and a tensor that is given other
     memory (`t.data = ...`, `set_`) needs a new handle. Building it copies the table to the device, waiting for that, and is
-    not for a captured region; clip() and norm() are (their workspace is allocated per call), and may run on any stream."""
+    not for a captured region; clip() and norm() are (their workspace is allocated per call, the table outlives the handle;
+    the tensors are the graph's inputs and the caller's to keep), and may run on any stream."""
 
     def __init__(self, grads, out=None):
         self.grads = list(grads)
@@ -208,6 +210,7 @@ class GradClip:
         if self.out is not self.grads:
             self._memory += [t.untyped_storage() for t in self.out]
         self._table, self._count = self._pieces()
+        self._captured = False
         self._stream = ops._raw_stream(self.device.index)
         self._parts = ops.call("vpt_grad_list_parts", self._count)
         self._in_place = int(all(o.data_ptr() == g.data_ptr() for g, o in zip(self.grads, self.out)))
@@ -232,8 +235,13 @@ class GradClip:
     def _run(self, max_norm: float, clip_value: float, count: int, want_norm: bool):
         with ops._on(self.device.index):
             st = ops._raw_stream(self.device.index)
-            if st != self._stream and self._table is not None and not torch.cuda.is_current_stream_capturing():
-                self._table.record_stream(torch.cuda.current_stream())
+            if self._table is not None:
+                if ops._capturing():
+                    if not self._captured:
+                        self._captured = True
+                        _CAPTURED.append(self._table)
+                elif st != self._stream:
+                    self._table.record_stream(torch.cuda.current_stream())
             table = None if self._table is None else self._table.data_ptr()
             if not want_norm:
                 ops.call("vpt_grad_list_clip", table, count, self._in_place, None, 0, 0.0, clip_value, None, st)
