@@ -225,3 +225,12 @@ def test_the_memory_of_the_table_stays(m, monkeypatch):
     mem = [t.untyped_storage().data_ptr() for t in (g, o)]
     g.data, o.data = z(40, d=F32), z(40, d=F32)
     assert {s.data_ptr() for s in c._memory} == set(mem)
+
+
+def test_no_handle_in_a_capture(m, monkeypatch):
+    """Its table is copied from the host; refused before that."""
+    ops, optim, _ = m
+    monkeypatch.setattr(ops, "_capturing", lambda: True, raising=False)
+    monkeypatch.setattr(optim.GradClip, "_pieces", lambda self: pytest.fail("a copy inside the capture"))
+    with pytest.raises(RuntimeError, match="captured"):
+        handle(optim, [z(4, d=F32)])._finish()

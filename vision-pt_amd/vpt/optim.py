@@ -165,8 +165,8 @@ class GradClip:
     overlap. The handle keeps the tensors, their memory as it was then, and a table of it on the device: gradients that are new
     tensors every step (`zero_grad(set_to_none=True)`) go through clip_grad_norm_ instead, and a tensor that is given other
     memory (`t.data = ...`, `set_`) needs a new handle. Building it copies the table to the device, waiting for that, and is
-    not for a captured region; clip() and norm() are (their workspace is allocated per call, the table outlives the handle;
-    the tensors are the graph's inputs and the caller's to keep), and may run on any stream."""
+    refused in a captured region; clip() and norm() are for one (their workspace is allocated per call, the table outlives
+    the handle; the tensors are the graph's inputs and the caller's to keep), and may run on any stream."""
 
     def __init__(self, grads, out=None):
         self.grads = list(grads)
@@ -206,6 +206,8 @@ class GradClip:
     def _finish(self):
         """The table of the checked tensors, and what it names: the memory stays this handle's, also when a tensor is given
         other memory meanwhile (`t.data = ...`)."""
+        if ops._capturing():
+            raise RuntimeError("GradClip: built inside a captured region (its table is copied from the host): build it before")
         self._memory = [t.untyped_storage() for t in self.grads]
         if self.out is not self.grads:
             self._memory += [t.untyped_storage() for t in self.out]
