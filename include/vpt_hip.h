@@ -346,7 +346,8 @@ int vpt_clip_coef(const float* part, int n, float max_norm, float* coef, float* 
  * gradients in tensors of their own: the caller cuts them into pieces of at most vpt_grad_list_piece() values and keeps the
  * table in device memory. norm: part[vpt_grad_list_parts(count)] = sums of squares (f64, fixed order). clip: norm_out (may be
  * null) = sqrt(sum of part's `parts` sums, of this table or of another); out = clamp(min(1, max_norm / (norm + 1e-6)) * g, +-clip_value), max_norm / clip_value 0: off;
- * out may be g (in_place: all are; a hint for caching, no more). g and out of a piece have its dtype (0 bf16, 1 f32, 2 f16) and alignment. */
+ * out may be g. cached: the results stay in the caches (0: they go past them, for more bytes than those hold); a
+ * hint, no more. g and out of a piece have its dtype (0 bf16, 1 f32, 2 f16) and alignment. */
 typedef struct {
   const void* g;
   void* out;
@@ -355,7 +356,7 @@ typedef struct {
 int vpt_grad_list_piece(void);
 int vpt_grad_list_parts(int count);
 int vpt_grad_list_norm(const void* pieces, int count, double* part, void* stream);
-int vpt_grad_list_clip(const void* pieces, int count, int in_place, const double* part, int parts, float max_norm,
+int vpt_grad_list_clip(const void* pieces, int count, int cached, const double* part, int parts, float max_norm,
                        float clip_value, float* norm_out, void* stream);
 int vpt_sf_lerp(void* y, const float* z, long n, float w, void* stream);
 /* EMA copy of the flat bf16 parameters (swa_utils.AveragedModel(get_ema_avg_fn(decay)), use_buffers=False;

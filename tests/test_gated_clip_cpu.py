@@ -234,3 +234,21 @@ def test_no_handle_in_a_capture(m, monkeypatch):
     monkeypatch.setattr(optim.GradClip, "_pieces", lambda self: pytest.fail("a copy inside the capture"))
     with pytest.raises(RuntimeError, match="captured"):
         handle(optim, [z(4, d=F32)])._finish()
+
+
+def test_streamed_by_bytes(m, monkeypatch):
+    """Results go past the caches where gradients and results are more bytes than those hold, however many tensors they are."""
+    ops, optim, _ = m
+    monkeypatch.setattr(ops, "_raw_stream", lambda index: 7)
+    monkeypatch.setattr(ops, "_capturing", lambda: False)
+
+    def cached(sizes, dtype, in_place=False):
+        flat = torch.empty(sum(sizes), dtype=dtype)
+        grads = list(flat.split(sizes))
+        c = handle(optim, grads, None if in_place else list(torch.empty_like(flat).split(sizes)))
+        c._finish()
+        return c._cached
+    assert cached([300] * 3000, BF16) == 1  # 1.8 MB in 3000 pieces
+    assert cached([16384] * 3000, BF16) == 1  # 98 MB and as much again
+    assert cached([70_000_000], BF16) == 0 and cached([35_000_000], F32) == 0
+    assert cached([70_000_000], BF16, in_place=True) == 1

@@ -198,21 +198,18 @@ extern "C" int vpt_grad_list_norm(const void* pieces, int count, double* part, v
   return VPT_OK;
 }
 
-extern "C" int vpt_grad_list_clip(const void* pieces, int count, int in_place, const double* part, int parts, float max_norm,
+extern "C" int vpt_grad_list_clip(const void* pieces, int count, int cached, const double* part, int parts, float max_norm,
                                   float clip_value, float* norm_out, void* stream) {
   VPT_CHECK_ARG(count >= 0 && (count == 0 || pieces), "vpt_grad_list_clip: bad table");
   VPT_CHECK_ARG(max_norm >= 0.f && clip_value >= 0.f, "vpt_grad_list_clip: max_norm, clip_value >= 0 (0: off)");
   VPT_CHECK_ARG((part && parts >= 1 && parts <= kBlocks && ((uintptr_t)part & 7) == 0) || (!part && max_norm == 0.f && !norm_out),
                 "vpt_grad_list_clip: a norm needs part, the parts doubles that vpt_grad_list_norm wrote");
-  // 2048 pieces are 64 or 128 MB, with as much output about what the 256-MB cache holds: beyond that, caching the clipped
-  // gradients drives out the ones still to be read (87 M f32 values into buffers of their own, norm and clip: 208 us
-  // cached, 172 us streamed). In place the stores go to lines that were just read.
   const dim3 grid(vpt_grad_list_parts(count));
-  if (!in_place && count > 2048)
-    hipLaunchKernelGGL(grad_list_clip_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, (const Piece*)pieces, count, part,
+  if (cached)
+    hipLaunchKernelGGL(grad_list_clip_kernel<false>, grid, dim3(256), 0, (hipStream_t)stream, (const Piece*)pieces, count, part,
                        parts, max_norm, clip_value, norm_out);
   else
-    hipLaunchKernelGGL(grad_list_clip_kernel<false>, grid, dim3(256), 0, (hipStream_t)stream, (const Piece*)pieces, count, part,
+    hipLaunchKernelGGL(grad_list_clip_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, (const Piece*)pieces, count, part,
                        parts, max_norm, clip_value, norm_out);
   VPT_LAUNCH_CHECK();
   return VPT_OK;
