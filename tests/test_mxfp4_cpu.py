@@ -157,3 +157,14 @@ def test_out_is_not_x(m):
     w = type("W", (), dict(shape=(64, 64), codes=torch.zeros(64, 64, dtype=torch.uint8), scales=torch.zeros(64, 4, dtype=torch.uint8)))
     with pytest.raises(ValueError, match="out is x"):
         m[0].linear_mxfp4(x, w, out=x)
+
+
+def test_numbers_are_no_matrices(m):
+    """A tensor without dims is refused as any other wrong shape."""
+    ops, mxfp4, _ = m
+    w = mxfp4.MXFP4Weight(*parts(16, 64), (16, 64))
+    u8, bf = torch.zeros((), dtype=U8), torch.zeros((), dtype=torch.bfloat16)
+    for call in (lambda: ops.mxfp4_dequantize(u8, u8, 64), lambda: ops.gemm_mxfp4(u8, u8, w), lambda: ops.linear_mxfp4_dgrad(bf, w),
+                 lambda: ops.linear_mxfp4(bf, w), lambda: ops.mxfp4_quantize(bf), lambda: ops.gated_norm_fwd(bf, bf)):
+        with pytest.raises(ValueError, match="shape"):
+            call()

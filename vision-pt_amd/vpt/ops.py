@@ -1476,7 +1476,7 @@ def mxfp4_quantize(x, codes=None, scales=None):
 def mxfp4_dequantize(codes, scales, K: int, out=None, dtype=BF16):
     """The values of an MXFP4 tensor as [M, K] bf16 (exact: a code has two significant bits) or f32."""
     _need(K >= 1, "mxfp4_dequantize: K >= 1")
-    M = codes.shape[0]
+    M = codes.shape[0] if codes.dim() else 0
     _mx_parts(codes, scales, M, K, "mxfp4_dequantize")
     if out is None:
         _need(dtype in _MX_OUT, "mxfp4_dequantize: dtype bf16 or f32")
@@ -1514,7 +1514,7 @@ def gemm_mxfp4(a_codes, a_scales, w, out=None, *, bias=None, resid=None, out_dty
     gives it, w a vpt.mxfp4.MXFP4Weight [N, K]. f32 accumulation, bias and residual added in f32, one rounding to out's type
     (bf16 or f32). `out` may be `resid` itself, and shares memory with no other operand. See csrc/mxfp4.hip."""
     N, K = w.shape
-    M = a_codes.shape[0]
+    M = a_codes.shape[0] if a_codes.dim() else 0
     _mx_parts(a_codes, a_scales, M, K, "gemm_mxfp4")
     out = _mx_out("gemm_mxfp4", M, N, a_codes.device, w, (("a_codes", a_codes), ("a_scales", a_scales)), bias, resid, out, out_dtype)
     dev = _gpu("gemm_mxfp4", a_codes, a_scales, w.codes, w.scales, out, bias, resid)
@@ -1568,8 +1568,8 @@ def linear_mxfp4_dgrad(dy, w, out=None):
     [M, K] bf16). W is dequantised to bf16 (exact) and goes through the bf16 GEMM, whose rows start at multiples of 16
     bytes, less than 2^22 values apart: N % 8 == 0 and K % 8 == 0, and dy and out with such rows."""
     N, K = w.shape
-    M = dy.shape[0]
     _rows2d(dy, "linear_mxfp4_dgrad", "dy", (BF16,))
+    M = dy.shape[0]
     if dy.shape[1] != N:
         raise ValueError(f"linear_mxfp4_dgrad: dy {tuple(dy.shape)} does not match W {w.shape}")
     if N % 8 or K % 8:
