@@ -382,3 +382,53 @@ def test_not_finite_vectors(ops, D, name, bad, R):
     for k, ref in (("dscale", wide["w_pre"] * P), ("dw_pre", ((1 + wide["scale"]) * P).sum(0)), ("dgate", 0.7 * wide["w_post"] * Q),
                    ("dw_post", (0.7 * wide["gate"] * Q).sum(0)), ("dshift", dy.double().view(G, R, D).sum(1))):
         same(getattr(got, k), ref, k)
+
+
+def passes(ops, G, R, D):
+    """Passes of the backward's blocks over their rows, from the workspace: blocks per group x 3 sums x D x 4 bytes."""
+    blocks = ops.call("vpt_gated_norm_bwd_workspace", G, R, D) // (12 * G * D)
+    at_once = 16 if D <= 384 else 4 if D <= 1536 else 1
+    return -(-(-(-R // blocks)) // at_once)
+
+
+@pytest.mark.parametrize("stream", [BF16, F32])
+@pytest.mark.parametrize("G,R,D,opts", [(1, 17000, 64, "pnGM"), (3, 11003, 136, "pngm"), (3, 1401, 768, "pnGM"), (2, 1537, 768, "pG"),
+                                        (2, 1031, 1280, "pngM"), (5, 823, 1288, "nM"), (2, 1111, 2048, "pnGM"), (3, 301, 4096, "pnGm"),
+                                        (1, 601, 10240, "pnGM"), (7, 601, 768, "pnGM")])
+def test_blocks_of_several_passes(ops, G, R, D, stream, opts):
+    """Rows enough that a block goes over several of them: sums kept from pass to pass, a last pass short of rows, groups that
+    end within a block's pass; forward and backward, with and without the stream's own gradient."""
+    assert passes(ops, G, R, D) >= 2
+    h, x, kw = make(G, R, D, stream, opts, seed=R)
+    x_new, y, rh, rx = check_fwd(ops, h, x, kw)
+    dy = rnd(G * R, D, seed=51) if y is not None else None
+    dxn = rnd(G * R, D, dtype=stream, seed=50)
+    got = check_bwd(ops, h, x_new, rh, rx, kw, dxn, dy)
+    again = ops.gated_norm_bwd(dy, dxn, h, x_new, rh, rx, **kw)
+    assert all(a is b or torch.equal(a, b) for a, b in zip(got, again))
+    if y is not None:
+        check_bwd(ops, h, x_new, rh, rx, kw, None, dy)
+
+
+@pytest.mark.parametrize("stream", [BF16, F32])
+@pytest.mark.parametrize("G,R,D", [(1, 17000, 64), (3, 1401, 768), (2, 1111, 2048)])
+def test_several_passes_strided_in_place(ops, G, R, D, stream):
+    """The same over rows of wider tensors, results over their inputs, and what lies around stays."""
+    assert passes(ops, G, R, D) >= 2
+    M = G * R
+    h, x, kw = make(G, R, D, stream, "pnGM", seed=9)
+    want = ops.gated_norm_fwd(h, x, **kw)
+    dy, dxn = rnd(M, D, seed=50), rnd(M, D, dtype=stream, seed=51)
+    grads = ops.gated_norm_bwd(dy, dxn, h, want[0], want[2], want[3], **kw)
+
+    def wide(t):
+        buf = torch.full((M + 2, D + 24), 9.0, dtype=t.dtype, device=DEV)
+        return buf, buf[1:M + 1, 8:D + 8].copy_(t)
+    (hb, hv), (xb, xv), (db, dv), (nb, nv) = wide(h), wide(x), wide(dy), wide(dxn)
+    f = ops.gated_norm_fwd(hv, xv, x_out=xv, **kw)
+    assert all(torch.equal(a, b) for a, b in zip(f, want))
+    got = ops.gated_norm_bwd(dv, nv, hv, xv, f[2], f[3], dh=hv, dx=nv, **kw)
+    assert all(torch.equal(a, b) for a, b in zip(got, grads))
+    for buf, v in ((hb, hv), (xb, xv), (db, dv), (nb, nv)):
+        v.fill_(9.0)
+        assert (buf == 9.0).all()
