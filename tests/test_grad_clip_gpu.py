@@ -218,3 +218,42 @@ def test_past_32_bits(optim):
     norm = optim.GradClip([g]).clip(8.5)
     assert norm.item() == math.sqrt(9 + 16 + 144 + 84 * 84)
     assert abs(g[1 << 31].item() - 8.4) < 0.04 and abs(g[0].item() - 0.3) < 0.002 and g[2:1000].abs().max().item() == 0
+
+
+def test_captured_and_the_handle_gone(optim):
+    """A graph's replays after its handle went and its memory was asked for again."""
+    import gc
+    data = [[rnd(n, F32, seed=10 * k + i) for i, n in enumerate((20000, 3, 40001))] for k in range(2)]
+    grads = [torch.empty_like(g) for g in data[0]]
+    out = [torch.empty_like(g) for g in grads]
+    handle = optim.GradClip(grads, out=out)
+    want = []
+    for d in data:
+        [g.copy_(t) for g, t in zip(grads, d)]
+        want.append([handle.clip(1.0).clone(), *(o.clone() for o in out)])
+    size = handle._table.numel()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = handle.clip(1.0)
+    del handle
+    gc.collect()
+    junk = [torch.full((size,), 255, dtype=torch.uint8, device=DEV) for _ in range(64)]
+    for k in (0, 1, 0):
+        [g.copy_(t) for g, t in zip(grads, data[k])]
+        [o.zero_() for o in out]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip([norm, *out], want[k]))
+    assert all((j == 255).all() for j in junk)
+
+
+def test_a_gradient_given_other_memory(optim):
+    """A handle's table names the memory its tensors had: that stays, and what lies elsewhere is left alone."""
+    g = rnd(30000, F32, seed=1)
+    handle, first = optim.GradClip([g]), g.detach().clone()
+    g.data = torch.full_like(g, 7.0)
+    torch.cuda.empty_cache()
+    others = [torch.full_like(g, 5.0) for _ in range(8)]
+    norm = handle.clip(1.0)
+    assert abs(norm.item() - norm64([first])) <= 2.0 ** -23 * norm64([first])
+    assert (g == 7.0).all() and all((o == 5.0).all() for o in others)
