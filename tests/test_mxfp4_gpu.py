@@ -425,3 +425,190 @@ def test_bias_anywhere(m, M, N, K, off):
     at = torch.empty(off + N, dtype=BF16, device=DEV)[off:].copy_(b)
     zero = ops.linear_mxfp4(x, w, out_dtype=F32)
     assert torch.equal(ops.linear_mxfp4(x, w, bias=at, out_dtype=F32), zero + b.float())
+
+
+# Sizes that the dispatch sends to each kernel of many rows, the last tile 4 or 8 rows high: 128 x 128 tiles (two steps along K,
+# whose scales go straight to registers, and five), 256 x 128 tiles, the 256 x 256 ring (24 steps and more).
+TILES = [(260, 1000, 200), (260, 1000, 520), (8200, 3080, 648), (3848, 4000, 3100)]
+GUARD = 300  # more rows than a tile has: what a tile would write behind row M lies in these
+
+
+def framed(M, N, dtype, off, fill):
+    """(buffer, [M, N] view of it): GUARD rows before and behind, columns beside."""
+    buf = torch.full((M + 2 * GUARD, N + 24), fill, dtype=dtype, device=DEV)
+    return buf, buf[GUARD:GUARD + M, off:off + N]
+
+
+def only_inside(buf, M, N, off, fill):
+    buf[GUARD:GUARD + M, off:off + N] = fill
+    return bool((buf == fill).all())
+
+
+def gaps(t, n):
+    return torch.full((t.shape[0], t.shape[1] + n), 255, dtype=torch.uint8, device=DEV)[:, n:].copy_(t)
+
+
+@pytest.mark.parametrize("M,N,K", TILES)
+@pytest.mark.parametrize("out_dtype", [BF16, F32])
+@pytest.mark.parametrize("off", [8, 1])
+def test_tiles_write_their_rows_alone(m, M, N, K, out_dtype, off):
+    """16-byte stores (off 8) and element by element (off 1): the result of a dense call, nothing written behind the last row,
+    before the first or beside the columns, nothing but the residual's own rows read; codes and scales with gaps; in place."""
+    ops, mxfp4 = m
+    x, wt, b, r, w, y = product(m, M, N, K, seed=N, out_dtype=out_dtype)
+    close(y, x, wt, b, r)
+    a, s = ops.mxfp4_quantize(x)
+    wg = mxfp4.MXFP4Weight(gaps(w.codes, 48), gaps(w.scales, 4), w.shape)
+    buf, out = framed(M, N, out_dtype, off, 5.0)
+    rbuf, rr = framed(M, N, BF16, off, float("nan"))
+    rr.copy_(r)
+    assert torch.equal(ops.gemm_mxfp4(gaps(a, 16), gaps(s, 4), wg, out, bias=b, resid=rr), y)
+    assert only_inside(buf, M, N, off, 5.0)
+    assert torch.equal(ops.linear_mxfp4(x, wg, bias=b, resid=rr, out=out), y) and only_inside(buf, M, N, off, 5.0)
+    rbuf.fill_(3.0)
+    if out_dtype == BF16:
+        rr.copy_(r)
+        assert torch.equal(ops.linear_mxfp4(x, w, bias=b, resid=rr, out=rr), y)
+    assert only_inside(rbuf, M, N, off, 3.0)
+    y0 = ops.linear_mxfp4(x, w, out_dtype=out_dtype)
+    assert torch.equal(ops.linear_mxfp4(x, w, out=out), y0) and only_inside(buf, M, N, off, 5.0)
+
+
+@pytest.mark.parametrize("M,N,K", TILES)
+def test_tiles_not_finite_blocks(m, M, N, K):
+    """As test_not_finite_blocks: scale byte 255 in every of a row's 4-step groups, in A and in W."""
+    ops, mxfp4 = m
+    x, wt = rnd(M, K, seed=1), rnd(N, K, seed=2)
+    clean = ops.linear_mxfp4(x, mxfp4.MXFP4Weight.quantize(wt))
+    x2, w2 = x.clone(), wt.clone()
+    rows = [0, 77, M // 2, M - 3, M - 1]
+    cols = [3, N // 2, N - 1]
+    for i, r in enumerate(rows):
+        x2[r, (i * K) // len(rows) + 5] = float("inf") if i % 2 else float("nan")
+    for i, c in enumerate(cols):
+        w2[c, K - 1 - (i * K) // len(cols)] = float("nan") if i % 2 else float("-inf")
+    y = ops.linear_mxfp4(x2, mxfp4.MXFP4Weight.quantize(w2))
+    mask = torch.zeros(M, N, dtype=torch.bool, device=DEV)
+    mask[rows] = True
+    mask[:, cols] = True
+    assert torch.equal(y.isnan(), mask) and torch.equal(y[~mask], clean[~mask])
+
+
+@pytest.mark.parametrize("M,N,K", TILES)
+def test_tiles_exact_integers(m, M, N, K):
+    """As test_exact_small_integers: multiples of 1/4 whose sums stay below 2^24 / 4 (36 per product, K <= 3100)."""
+    ops, mxfp4 = m
+    g = torch.Generator().manual_seed(M)
+
+    def pick(rows, cols):
+        v = torch.cat([GRID, -GRID])[torch.randint(0, 16, (rows, cols), generator=g)]
+        v[:, ::32] = 4.0  # the block's scale
+        return v.float().to(DEV)
+    x, wt = pick(M, K), pick(N, K)
+    y = ops.linear_mxfp4(x, mxfp4.MXFP4Weight.quantize(wt), out_dtype=F32)
+    assert torch.equal(y.double(), x.double() @ wt.double().t())
+
+
+@pytest.mark.parametrize("M,N,K", TILES)
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_tiles_input_types(m, M, N, K, dtype):
+    ops, mxfp4 = m
+    x, wt = rnd(M, K, dtype=dtype, seed=4, spread=1.0), rnd(N, K, dtype=dtype, seed=5)
+    w = mxfp4.MXFP4Weight.quantize(wt)
+    y = ops.linear_mxfp4(x, w)
+    close(y, x, wt, None, None)
+    assert torch.equal(y, ops.gemm_mxfp4(*ops.mxfp4_quantize(x), w))
+
+
+@pytest.mark.parametrize("M,N,K", TILES)
+def test_tiles_streams_and_graphs(m, M, N, K):
+    """On another stream, captured twice, replayed with new inputs between eager calls: the same bits."""
+    ops, mxfp4 = m
+    w, b = mxfp4.MXFP4Weight.quantize(rnd(N, K, seed=1)), rnd(N, seed=2)
+    xs, r = [rnd(M, K, seed=10 + i) for i in range(3)], rnd(M, N, seed=3)
+    want = [ops.linear_mxfp4(x, w, bias=b, resid=r) for x in xs]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = ops.linear_mxfp4(xs[0], w, bias=b, resid=r)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want[0])
+    x, graphs, res = xs[0].clone(), [], []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            res.append(ops.linear_mxfp4(x, w, bias=b, resid=r))
+    for i in (1, 2, 0):
+        x.copy_(xs[i])
+        [g.replay() for g in graphs]
+        eager = ops.linear_mxfp4(xs[i - 1], w, bias=b, resid=r)
+        torch.cuda.synchronize()
+        assert all(torch.equal(t, want[i]) for t in res) and torch.equal(eager, want[i - 1])
+
+
+@pytest.mark.parametrize("what", ["out", "out f32", "resid", "codes", "scales", "W codes", "W scales"])
+def test_rows_far_apart(m, what):
+    """An operand whose rows lie 4 MB apart and more, at a size past the few-row kernel's: the kernel with 64-bit addresses,
+    against the definition, and what lies around the result stays."""
+    ops, mxfp4 = m
+    M, N, K = (2000, 140, 300) if what[0] == "W" else (130, 1500, 300)
+    dtype = F32 if what == "out f32" else BF16
+    x, wt, b, r = rnd(M, K, seed=1, spread=1.0), rnd(N, K, dtype=F32, seed=2, spread=1.0), rnd(N, seed=3), rnd(M, N, seed=4)
+    w = mxfp4.MXFP4Weight.quantize(wt)
+    a, s = ops.mxfp4_quantize(x)
+    c, ws = w.codes, w.scales
+
+    def far(t, fill):
+        """t in rows of 4 MB of one buffer, a row of it free before and behind."""
+        buf = torch.full((t.shape[0] + 2, (1 << 22) // t.element_size()), fill, dtype=t.dtype, device=DEV)
+        return buf, buf[1:-1, 64:64 + t.shape[1]].copy_(t)
+    buf, out = None, None
+    if what.startswith("out"):
+        buf, out = far(torch.zeros(M, N, dtype=dtype, device=DEV), 5.0)
+    elif what == "resid":
+        _, r = far(r, float("nan"))
+    elif what == "codes":
+        _, a = far(a, 255)
+    elif what == "scales":
+        _, s = far(s, 255)
+    elif what == "W codes":
+        _, c = far(c, 255)
+    else:
+        _, ws = far(ws, 255)
+    y = ops.gemm_mxfp4(a, s, mxfp4.MXFP4Weight(c, ws, (N, K)), out, bias=b, resid=r, out_dtype=dtype)
+    close(y, x, wt, b, r)
+    assert torch.equal(ops.gemm_mxfp4(a, s, mxfp4.MXFP4Weight(c, ws, (N, K)), out, bias=b, resid=r, out_dtype=dtype), y)
+    if buf is not None:
+        out.fill_(5.0)
+        assert (buf == 5.0).all()
+
+
+def test_more_rows_than_a_launch(m):
+    """2^27 + 9 rows of 128 values: quantisation and dequantisation take several launches; the rows around their border and the
+    last ones as on their own, zeros elsewhere."""
+    ops, _ = m
+    M, K = (1 << 27) + 9, 128
+    x = torch.zeros(M, K, dtype=BF16, device=DEV)  # 34 GB
+    at = torch.tensor([0, 1, (1 << 26) + 3, (1 << 27) - 2, (1 << 27) - 1, 1 << 27, (1 << 27) + 1, M - 1], device=DEV)
+    x[at] = rnd(len(at), K, seed=8, spread=2.0)
+    codes, scales = ops.mxfp4_quantize(x)
+    want = ops.mxfp4_quantize(x[at].contiguous())
+    assert torch.equal(codes[at], want[0]) and torch.equal(scales[at], want[1])
+    back = ops.mxfp4_dequantize(codes, scales, K, out=x)
+    assert torch.equal(back[at], ops.mxfp4_dequantize(*want, K))
+    back[at], codes[at], scales[at] = 0, 0, 0
+    assert not any(t.any() for part in (back, codes, scales) for t in part.split(1 << 24))
+
+
+@pytest.mark.parametrize("K", [130, 3100])
+def test_streamed_tiles_write_their_rows_alone(m, K):
+    """Results past what the cache holds (stores that leave no copy in it), from the 256 x 128 tiles and from the ring: as above."""
+    ops, mxfp4 = m
+    M, N = 16392, 4104
+    x, w, b = rnd(M, K, seed=1, spread=1.0), mxfp4.MXFP4Weight.quantize(rnd(N, K, dtype=F32, seed=2)), rnd(N, seed=3)
+    y = ops.linear_mxfp4(x, w, bias=b, out_dtype=F32)
+    at = torch.tensor([0, 15, 16, 255, 256, 4095, M // 2, M - 9, M - 8, M - 1], device=DEV)
+    close(y[at], x[at], rnd(N, K, dtype=F32, seed=2), b, None)
+    buf, out = framed(M, N, F32, 8, 5.0)
+    assert torch.equal(ops.linear_mxfp4(x, w, bias=b, out=out), y)
+    assert only_inside(buf, M, N, 8, 5.0)

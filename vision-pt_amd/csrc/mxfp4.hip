@@ -225,8 +225,9 @@ __device__ __forceinline__ floatx4 mx_mfma_at(uint4 a, uint4 b, floatx4 c, uint3
 
 // acc[i][j][e]: row 16 i + (lane & 15), column 32 (j >> 1) + 8 (lane >> 4) + 4 (j & 1) + e of the wave's tile, which starts at
 // (row0, col0) of the block's at (m0, n0). VEC (N % 8 == 0, 16-byte rows): 16-byte buffer stores whose per-store part is one
-// scalar; rows past M lie behind the buffer's end, columns past N get an offset there, and the hardware drops them. Otherwise
-// element by element.
+// scalar; rows past M lie behind the buffer's end, columns past N get an offset there, and the hardware drops them (the
+// tests frame results of every kernel by more rows than a tile has, with last tiles of 4 and 8 rows). Otherwise element by
+// element.
 template <bool VEC, int AUX, int MI, int NP>
 __device__ __forceinline__ void mx_epilogue(const MxArgs& g, const floatx4 (&acc)[MI][2 * NP], int lane, int m0, int n0, int row0,
                                             int col0, const float (&bias)[NP][8]) {
