@@ -169,9 +169,12 @@ __device__ __forceinline__ floatx4 mx_mfma(uint4 a, uint4 b, floatx4 c, uint32_t
 // The product is taken transposed, W's fragment first, so that a lane holds 4 consecutive columns of one output row; W's rows
 // lie in LDS in an order (mx_wrow) that makes the columns of two fragments neighbours: 16-byte stores from registers.
 // What bounds it: 1.27 us per step of a CU's two blocks, of which the MFMAs need 0.6 at the 7.0 PFLOP/s that the instruction
-// reaches on random operands (9.8 on zeros); the rest is fragment reads (64 bytes a clock) and LDS-DMA, and for short
-// reductions the stores: 33360 x 4096 x 768 takes 98 us, 67 without its 273 MB of stores. 17568 x 2304 x 768 31 us,
-// 4224 x 1280 x 5120 (128-row tiles) 29 us.
+// reaches on random operands (9.8 on zeros). No unit is full: counters at 33360 x 4096 x 768 give MFMA busy 0.22, LDS reads
+// 0.11 without bank conflicts, and waves that wait 0.39 of their time to issue and 0.29 for memory and barriers. Short
+// reductions are bound by the stores: that product takes 101 us (105 to 114 with a bias), 67 without its 273 MB of
+// stores, which as half lines past the cache write 398 MB. 17568 x 2304 x 768 34 us; 4224 x 1280 x 5120 (128-row
+// tiles) 31 us, 36 with a residual: its loads wait behind the stores of the fragment before (17568 x 2304 x 768 with one 71,
+// 33360 x 4096 x 768 198).
 constexpr int MXST = 3;
 template <int TM> constexpr int mx_stage() { return (TM + 128) * 64; }               // 24 / 16 KB
 template <int TM> constexpr int mx_lds() { return MXST * mx_stage<TM>() + (TM + 128) * 16; }  // 78 / 52 KB
@@ -440,7 +443,7 @@ __global__ __launch_bounds__(256, 2) void mx_tile_kernel(MxArgs g) {
 // A stage is refilled in L_t, after both groups' L_t-1 closed with lgkmcnt(0) and a barrier; a step's pieces of all waves have
 // landed one barrier before the first group reads them. The scales' buffer (one, 16 bytes per row) is read in L_4c and
 // refilled from L_4c+1 on; its piece has landed where step 4c + 4's are waited for.
-// 1.02 us per step: 8192^3 in 294 us, 3.7 PFLOP/s. Wider waves (four of 128 x 128, a third less LDS reading, fragments a step
+// 1.02 us per step: 8192^3 in 286 to 307 us, 3.6 to 3.8 PFLOP/s, MFMA busy 0.48, LDS reads 0.23. Wider waves (four of 128 x 128, a third less LDS reading, fragments a step
 // ahead in registers) took 1.16: one wave per SIMD leaves its waits uncovered.
 constexpr int MXR_ST = 4, MXR_STG = 512 * 64;
 constexpr int mx_ring_lds() { return MXR_ST * MXR_STG + 512 * 16; }  // 136 KB
@@ -546,8 +549,9 @@ __global__ __launch_bounds__(512, 1) void mx_ring_kernel(MxArgs g) {
 // With few rows the product is a pass over W: each wave takes every fourth 128-deep step, its 16 rows of W straight from
 // memory into registers (four steps' loads in flight), and the four partial sums meet in LDS in a fixed order. FUSE: the block
 // quantises its rows of x itself, into LDS (M <= 16; the same codes as mx_quantize_kernel), and saves a launch. One row
-// of 2304 x 768: 2.5 us in a graph; of 10240 x 5120: 10 us, 2.8 TB/s of codes, bound by the latency of its few loads in
-// flight (8 instead of 4 per wave, or the first ones before x is quantised, were slower).
+// of 2304 x 768: 2.5 us in a graph; of 10240 x 5120: 10 us, 2.8 TB/s of codes, its waves waiting for memory 0.68 of their
+// time with few loads in flight, each of half a line of its row (8 loads instead of 4 per wave, or the first ones before x is
+// quantised, were slower).
 struct MxX {
   const void* x; long ldx;
   int K;

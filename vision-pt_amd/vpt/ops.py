@@ -1529,7 +1529,8 @@ def gemm_mxfp4(a_codes, a_scales, w, out=None, *, bias=None, resid=None, out_dty
 def linear_mxfp4(x, w, bias=None, resid=None, out=None, out_dtype=BF16):
     """y = q(x) . W^T (+ bias) (+ resid): nn.Linear on an MXFP4 weight with its input quantised to MXFP4 on the way
     (x [M, K] bf16, f16 or f32; w a vpt.mxfp4.MXFP4Weight [N, K]): mxfp4_quantize and gemm_mxfp4, in one launch for a few rows.
-    y is bf16 or f32; `out` may be `resid` itself, and shares memory with no other operand (blocks read x after others wrote)."""
+    y is bf16 or f32; `out` may be `resid` itself, and shares memory with no other operand (blocks read x after others wrote).
+    As every call here it records nothing for autograd: the gradient of x is linear_mxfp4_dgrad, W has none."""
     _rows2d(x, "linear_mxfp4", "x", _MX_DTYPES)
     M, K = x.shape
     N = w.shape[0]
@@ -1656,7 +1657,8 @@ def gated_norm_fwd(h, x, *, w_post=None, w_pre=None, gate=None, scale=None, shif
     [D], or [groups, D] with one row for each of `groups` equal runs of rows (a sample's tokens); rows of a wider tensor do.
     y is the norm of x_new as it is stored. D % 8 == 0, D <= 10240, rows at multiples of 16 bytes. `x_out` and `y` may each be
     x or h itself, and share no other memory with what is read or with each other.
-    Returns (x_new, y, rstd_post, rstd_pre), the last two f32 [M] for gated_norm_bwd; None where there is no such norm."""
+    Returns (x_new, y, rstd_post, rstd_pre), the last two f32 [M] for gated_norm_bwd; None where there is no such norm. Nothing
+    is recorded for autograd."""
     _rows2d(h, "gated_norm_fwd", "h", _BF16)
     M, D = h.shape
     _gn_params("gated_norm_fwd", D, M, groups, w_post, w_pre, gate, scale, shift)

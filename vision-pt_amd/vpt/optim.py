@@ -284,7 +284,9 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
                     clip_value: float | None = None) -> torch.Tensor:
     """torch.nn.utils.clip_grad_norm_ over parameters' .grad (its positions; norm_type 2 alone), then clip_grad_value_ when
     clip_value is given, in place. Parameters without a gradient are left out; error_if_nonfinite reads the norm back before
-    anything is scaled."""
+    anything is scaled. Every call builds the gradients' table (0.5 ms of the host for 226 of them, 2.1 ms for 1400) and copies
+    it, which waits for all work queued on the device; torch's function does not wait. Gradients that stay where they are go
+    through a GradClip kept over the steps, which neither builds nor waits."""
     if float(norm_type) != 2.0:
         raise ValueError(f"clip_grad_norm_: norm_type {norm_type}: the L2 norm (2.0) is the only one")
     params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
