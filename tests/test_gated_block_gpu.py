@@ -311,3 +311,53 @@ def test_stacks_on_mxfp4(m):
                     (X.shape[1] + 32) * 2.0 ** -23 * (X.abs() @ W.abs().t() + lin.scale * (X.abs() @ down.abs().t()) @ up.abs().t())
                 assert ((got.double() - ref).abs() <= tol).all()
     assert all(torch.equal(p, q) and torch.isfinite(p.float()).all() and p.float().abs().max() > 0 for p, q in zip(*res))
+
+
+def test_sdxl_block_captured(m):
+    """Two transformer blocks on MXFP4 bases, forward and backward captured each in a graph of its own, replayed at once on two
+    streams with new inputs while an eager step of a third runs: the eager bits (bases, slabs and tickets are a graph's own)."""
+    from vpt import sdxl
+    ops, mx, _ = m
+    dim, cdim, rank = 256, 512, 16
+    shapes = {t: (dim, cdim if t in ("attn2.to_k", "attn2.to_v") else dim) for t in sdxl.TARGETS}
+    shapes["ff.net.0.proj"], shapes["ff.net.2"] = (8 * dim, dim), (dim, 4 * dim)
+
+    def block(seed):
+        sd = {}
+        for i, (t, (n, k)) in enumerate(shapes.items()):
+            sd[f"{t}.linear.weight"] = mx.MXFP4Weight.quantize(rnd(n, k, seed=seed + i, scale=k ** -0.5))
+            sd[f"{t}.lora_down.weight"], sd[f"{t}.lora_up.weight"] = (rnd(*s, seed=seed + 20 + i, scale=0.05) for s in ((rank, k), (n, rank)))
+        for k in ("norm1", "norm2", "norm3"):
+            sd[f"{k}.weight"], sd[f"{k}.bias"] = torch.ones(dim, device=DEV), torch.zeros(dim, device=DEV)
+        return sdxl.SDXLTransformerBlock(dim, 4, cdim, rank, 16.0, sd)
+
+    def inputs(seed):
+        return [rnd(2 * 80, dim, seed=seed), rnd(2 * 20, cdim, seed=seed + 1), rnd(2 * 80, dim, seed=seed + 2, scale=0.1)]
+
+    def step(blk, x, ctx, dy):
+        grads = [g for lin in blk.lin.values() for g in (lin.g_up, lin.g_down)]
+        for g in grads:
+            g.zero_()
+        y = blk.forward(x, ctx, 2, 80, 20)
+        return [y, *blk.backward(dy), *grads]
+    blks, ins = [block(100 * k) for k in range(3)], [[inputs(1000 * k + 10 * i) for i in range(3)] for k in range(2)]
+    want = [[[t.clone() for t in step(b, *i)] for i in per] for b, per in zip(blks, ins)]
+    third = [t.clone() for t in step(blks[2], *ins[0][0])]
+    bufs, graphs, res = [[t.clone() for t in per[0]] for per in ins], [], []
+    for b, buf in zip(blks, bufs):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            res.append(step(b, *buf))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for k in (1, 2, 0, 1):
+        for buf, per in zip(bufs, ins):
+            for t, v in zip(buf, per[k]):
+                t.copy_(v)
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        eager = step(blks[2], *ins[0][0])
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for r, w in zip(res, want) for p, q in zip(r, w[k]))
+        assert all(torch.equal(p, q) for p, q in zip(eager, third))
